@@ -540,6 +540,94 @@ int lap_argmax_rows(const void* x, int64_t x_row_stride, int rows, int V, int dt
                     void* copy, lap_stream_t stream);
 
 /* ======================================================================= *
+ * Packed prompts: prompts of different lengths in one pass.  No counterpart  *
+ * in the reference, which prefills one length per batch                      *
+ * (aq_evaluation.py:150-155, 279-322); each sequence gets what it would get  *
+ * alone.                                                                     *
+ * ======================================================================= *
+ * lap_prompt_shape: the tile shape that the calls below take for `total`
+ * packed tokens of B sequences, no sequence with more than max_keys cached and
+ * new tokens: tokens per tile, an upper bound of the tiles, and the parts that
+ * a tile's keys are split into (host arithmetic, no device call). */
+int lap_prompt_shape(int total, int B, int max_keys, int Hq, int Hkv, int D,
+                     int* tokens_per_tile, int* n_tiles, int* nsplit);
+/* Tables from device lengths (B up to 4096; a length below zero counts as zero, tokens
+ * past `total` are cut off):
+ *   starts  int32 [B + 1] first packed token of each sequence, and of none
+ *   seq     int32 [total] sequence of a packed token, -1 behind the last one
+ *   pos     int64 [total] its cache row: cached_lens[b] (NULL: 0) + place among the new
+ *   tiles   int32 [n_tiles][4], or NULL: (first packed token, tokens, sequence, cache
+ *           row of the first), most keys first, then empty ones; 16-byte aligned,
+ *           n_tiles >= total / tokens_per_tile + min(B, total) */
+int lap_pack_prompts(const int32_t* new_lens, const int32_t* cached_lens, int B, int total,
+                     int tokens_per_tile, int n_tiles, int32_t* starts, int32_t* seq,
+                     int64_t* pos, int32_t* tiles, lap_stream_t stream);
+/* Norms of q and k per head, rotary embedding and cache append of `tokens` tokens
+ * (replaces apply_rotary_pos_emb and _kv_cache_append, aq_evaluation.py:296-305 and
+ * 65-112, and the head norms that a model may have before them):
+ *   y = w * x * rsqrt(mean(x^2) + eps); out = y * cos + rotate_half(y) * sin
+ * in fp32, rounded once; q_weight / k_weight [D] NULL: no norm, and the roundings of
+ * lap_rope_append (bit-identical to it).
+ *   q  [tokens][Hq][D]  strides (q_st, q_sh, 1);  k, v [tokens][Hkv][D] likewise
+ *   cos, sin [tokens][D], row stride cs_st (0: one row for all)
+ *   seq  int32 [tokens] (-1 or >= B: the token is left out), NULL: token i is sequence i
+ *   pos  int64 [tokens]; keys outside [0, t_cap) are not written
+ * rope(q) goes to q_out [tokens][Hq][D] (contiguous), rope(k) and v to the caches at
+ * (seq, pos).  D a multiple of 16 up to 256; rows 16-byte aligned. */
+int lap_qk_rope_append(const void* q, int64_t q_st, int64_t q_sh,
+                       const void* k, int64_t k_st, int64_t k_sh,
+                       const void* v, int64_t v_st, int64_t v_sh,
+                       const void* cos, const void* sin, int64_t cs_st,
+                       const void* q_weight, float q_eps, const void* k_weight, float k_eps,
+                       int dtype, int64_t tokens, int B, int Hq, int Hkv, int D,
+                       const int32_t* seq, const int64_t* pos,
+                       void* cache_k, int64_t ck_sb, int64_t ck_sh, int64_t ck_st,
+                       void* cache_v, int64_t cv_sb, int64_t cv_sh, int64_t cv_st,
+                       int t_cap, void* q_out, lap_stream_t stream);
+/* Causal attention of prompts over their caches (replaces SDPA over the prompt,
+ * laprune/attention.py:66-73, aq_evaluation.py:279-322): token i of a sequence with
+ * `cached` earlier tokens sees keys [0, cached + i],
+ *   o[i,h] = sum_t softmax_t(scale * q[i,h].K[b,h/G,t]) V[b,h/G,t]
+ * in fp32 but for the weights, which enter the second product in the data type.  A value
+ * in a row that a token does not see never reaches it, finite or not; weights that sum
+ * to zero give zeros.
+ *   tiles non-NULL: q, out [Tq][Hq][D] packed, the tiles of lap_pack_prompts; rows
+ *           of no sequence are not written.  tiles NULL: q, out [B][Tq][Hq][D], every
+ *           sequence's Tq tokens at the end of Tk keys (Tq <= Tk).
+ *   K/V     [B][Hkv][Tk][D] strides (sb, sh, st, 1); no row past Tk is read
+ *   tokens_per_tile, nsplit   of lap_prompt_shape; max_keys as given to it
+ *   workspace   for nsplit > 1: lap_prompt_attention_workspace_size(tokens, ...), tokens =
+ *           Tq (packed) or B * Tq.  Calls that share one must be ordered.
+ * D 64, 128 or 256, fp16/bf16, Hq / Hkv up to 256, every row 16-byte aligned. */
+int lap_prompt_attention_workspace_size(int64_t tokens, int Hq, int D, int nsplit, size_t* bytes);
+int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                         const void* keys, const void* vals,
+                         int64_t k_sb, int64_t k_sh, int64_t k_st,
+                         int64_t v_sb, int64_t v_sh, int64_t v_st,
+                         int dtype, int B, int Hq, int Hkv, int D, int Tq, int Tk,
+                         const int32_t* tiles, int n_tiles, int tokens_per_tile, int nsplit,
+                         int max_keys, float scale,
+                         void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                         void* workspace, size_t workspace_bytes, lap_stream_t stream);
+
+/* Dense decode of a batch whose sequences begin with the same `prefix` tokens (no
+ * counterpart in the reference; lap_dense_attn_decode and the dense form of
+ * lap_sparse_attn_decode_ragged read every sequence's own copy).  Keys [0, prefix) are
+ * read once, from sequence 0's rows, for all sequences; keys [prefix, len) are each
+ * sequence's own.  len = min(plans[b].t_total, T), or T where plans is NULL; a sequence
+ * shorter than the prefix sees len keys of it.  Other arguments and the output as
+ * lap_dense_attn_decode; q and K/V rows 16-byte aligned, Hq / Hkv up to 256. */
+int lap_shared_attn_decode_workspace_size(int B, int Hq, int Hkv, int D, int T, int prefix,
+                                          size_t* bytes);
+int lap_shared_attn_decode(const void* q, int64_t q_sb, int64_t q_sh,
+                           const void* keys, const void* vals, int dtype,
+                           int B, int Hq, int Hkv, int T, int D,
+                           int64_t k_sb, int64_t k_sh, int64_t k_st,
+                           int64_t v_sb, int64_t v_sh, int64_t v_st,
+                           int prefix, const lap_row_plan* plans, float scale, void* out,
+                           void* workspace, size_t workspace_bytes, lap_stream_t stream);
+
+/* ======================================================================= *
  * Diagnostics: measurement kernels (no counterpart in the reference; not  *
  * on the path and never called by it).                                    *
  * They time what the fused G = 4 scorer's launch shape costs before any   *

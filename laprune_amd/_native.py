@@ -102,6 +102,18 @@ SIGNATURES = {
                         vp, i64, i64, i64, vp, vp],
     "lap_encode_keys_ranges": [vp, i32, i64, i64, i64, i32, i32, vp, i32, i32, i32, vp, i32, i32,
                                vp, sz, vp, i64, i64, i64, vp],
+    "lap_prompt_shape": [i32, i32, i32, i32, i32, i32, pint, pint, pint],
+    "lap_pack_prompts": [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp],
+    "lap_qk_rope_append": [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp, i64, vp, f32, vp, f32,
+                           i32, i64, i32, i32, i32, i32, vp, vp, vp, i64, i64, i64, vp, i64, i64,
+                           i64, i32, vp, vp],
+    "lap_prompt_attention_workspace_size": [i64, i32, i32, i32, psz],
+    "lap_prompt_attention": [vp, i64, i64, i64, vp, vp, i64, i64, i64, i64, i64, i64, i32, i32,
+                             i32, i32, i32, i32, i32, vp, i32, i32, i32, i32, f32, vp, i64, i64,
+                             i64, vp, sz, vp],
+    "lap_shared_attn_decode_workspace_size": [i32, i32, i32, i32, i32, i32, psz],
+    "lap_shared_attn_decode": [vp, i64, i64, vp, vp, i32, i32, i32, i32, i32, i32, i64, i64, i64,
+                               i64, i64, i64, i32, vp, f32, vp, vp, sz, vp],
     "lap_floor_empty": [i32, i32, vp],
     "lap_floor_stream": [vp, vp, i64, i64, i32, i32, i32, vp, vp],
 }

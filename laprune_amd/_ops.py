@@ -17,6 +17,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -24,6 +25,24 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblaprune_torch.so"
 
 _lock = threading.Lock()
 _ops = None
+
+# looked up once: every wrapped call of an eager step asks them
+_compiling, _grad_on = torch.compiler.is_compiling, torch.is_grad_enabled
+_transforms, _modes = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
+_trace = torch._C._get_tracing_state
+
+
+def untraced() -> bool:
+    """Whether no compiler, function transform (vmap, jvp), forward-mode level, dispatch
+    mode (fake tensors, op counters) or trace looks at the calling ops, all of which a
+    kernel call would pass by."""
+    return not (_compiling() or forward_ad._current_level >= 0 or _transforms() is not None or
+                _modes() or _trace() is not None)
+
+
+def unwatched() -> bool:
+    """Whether the calling ops only have to compute: untraced, and no gradients."""
+    return not _grad_on() and untraced()
 
 
 def ops():

@@ -7,15 +7,24 @@ mask, native GQA, output ``[B, T, H*D]`` through ``out_proj`` when given.
 A single query without a mask or down-projections (decode; the reference's
 ``num_queries == 1`` branch, :62-65) runs the split-K flash-decode kernel
 (``lap_dense_attn_decode``): fp16/bf16, head dim 64/128/256, 1/2/4/8 query
-heads per KV head, K/V rows 16-byte aligned.  Every other case (prefill with
-the causal or tail-causal mask, an explicit mask, down-projections, shapes
-outside the kernel's contract) runs ``scaled_dot_product_attention`` exactly
-as the reference does.
+heads per KV head, K/V rows 16-byte aligned.  Several queries without a mask
+(prefill, with the causal or tail-causal mask of :66-73) run the prompt
+kernel (``lap_prompt_attention``) on rows of the same kind when no gradient is
+needed.  Every other case (an explicit mask, shapes outside the kernels'
+contract) runs ``scaled_dot_product_attention`` exactly as the reference does.
+
+:func:`prompt_attention` is that kernel for packed prompts of different lengths
+over their caches.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
+
+from . import _native as N
+from ._ops import ops, untraced
 
 
 def _tail_causal_mask(num_queries: int, num_keys: int, dtype, device) -> torch.Tensor:
@@ -51,6 +60,78 @@ def _decode_kernel_fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bo
     return True
 
 
+def _needs_grad(*ts: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+
+
+def _rows16(t: torch.Tensor) -> bool:
+    """Rows of contiguous values that start at multiples of 16 bytes."""
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and
+            all(s % 8 == 0 for s in t.stride()[:-1]))
+
+
+def _prompt_kernel_fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
+    """Several queries [B, Hq, Tq, D] at the end of [B, Hkv, Tk, D] keys, for the
+    prompt kernel."""
+    return (q.is_cuda and k.is_cuda and v.is_cuda and q.dim() == 4 and k.dim() == 4 and
+            v.shape == k.shape and q.dtype in (torch.float16, torch.bfloat16) and
+            k.dtype == q.dtype and v.dtype == q.dtype and q.device == k.device == v.device and
+            q.shape[0] == k.shape[0] > 0 and k.shape[1] > 0 and q.shape[3] == k.shape[3] and
+            q.shape[3] in (64, 128, 256) and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and
+            q.shape[1] // k.shape[1] <= 256 and 0 < q.shape[2] <= k.shape[2] and
+            all(type(t) in (torch.Tensor, torch.nn.Parameter) and _rows16(t) for t in (q, k, v)) and
+            untraced() and not _needs_grad(q, k, v))
+
+
+def _prompt_launch(q, k, v, tiles, shape, max_keys: int, scale: float, out) -> None:
+    Hq, D = q.shape[-2:]
+    tokens = q.numel() // (Hq * D)
+    ws = None
+    if shape[2] > 1:
+        need = N.size_query("lap_prompt_attention_workspace_size", tokens, Hq, D, shape[2])
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ops().prompt_attention(q, k, v, tiles, shape[0], shape[2], max_keys, scale, out, ws)
+
+
+def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, plan,
+                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed prompts over their caches.
+
+    query [n, Hq, D]: the packed tokens' post-RoPE queries; keys, values
+    [B, Hkv, T, D]: each sequence's cache, the new tokens' rows included (any strides
+    between rows); plan: :func:`laprune_amd.packed.pack_prompts` of the n tokens with
+    these head counts.  A token at position p of its sequence sees cache rows
+    [0, p].  Returns [n, Hq, D] (``out`` if given; rows of no sequence are left as
+    they are).  scale: 1/sqrt(D) by default.  fp16/bf16, D 64/128/256; no gradients."""
+    q, k, v = query, keys, values
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise RuntimeError("prompt_attention: tensors must be on CUDA (ROCm) devices")
+    if _needs_grad(q, k, v):
+        raise RuntimeError("prompt_attention computes no gradients: call it under no_grad, or "
+                           "do_sdpa_attn for tensors that require them")
+    if q.dim() != 3 or k.dim() != 4 or v.shape != k.shape:
+        raise RuntimeError("prompt_attention: query [n, Hq, D], keys and values [B, Hkv, T, D]")
+    if plan.heads is None:
+        raise RuntimeError("prompt_attention: the plan was made without head counts")
+    if plan.heads != (q.shape[1], k.shape[1], q.shape[2]) or q.shape[2] != k.shape[3]:
+        raise RuntimeError(f"prompt_attention: the plan is for (Hq, Hkv, D) = {plan.heads}, got "
+                           f"({q.shape[1]}, {k.shape[1]}, {q.shape[2]})")
+    if plan.total != q.shape[0] or plan.B != k.shape[0]:
+        raise RuntimeError(f"prompt_attention: a plan of {plan.total} tokens of {plan.B} sequences, "
+                           f"got {q.shape[0]} of {k.shape[0]}")
+    if plan.lens is not None and plan.max_keys > k.shape[2] and plan.total:
+        raise RuntimeError(f"prompt_attention: {plan.max_keys} keys exceed the {k.shape[2]} rows "
+                           "of the caches")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise RuntimeError("prompt_attention: out must be like query")
+    if plan.total:
+        _prompt_launch(q, k, v, plan.tiles, plan.shape, plan.max_keys,
+                       1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale), out)
+    return out
+
+
 def do_sdpa_attn(query, key, value, cos=None, sin=None, out_proj=None, query_down_proj=None,
                  key_down_proj=None, mask=None, already_rope: bool = False):
     """Attention over post-RoPE Q/K with native GQA caches."""
@@ -73,6 +154,14 @@ def do_sdpa_attn(query, key, value, cos=None, sin=None, out_proj=None, query_dow
             and key_down_proj is None and _decode_kernel_fits(q, k, v)):
         from .aq_kernels import _impl
         output = _impl.dense_attn_decode(q, k, v)
+    elif mask is None and num_queries > 1 and _prompt_kernel_fits(q, k, v):
+        from .packed import prompt_shape
+        B, Hq, Tq, D = q.shape
+        output = q.new_empty((B, Tq, Hq, D))
+        _prompt_launch(q.transpose(1, 2), k, v, None,
+                       prompt_shape(B * Tq, B, k.shape[2], Hq, k.shape[1], D), k.shape[2],
+                       1.0 / math.sqrt(D), output)
+        output = output.transpose(1, 2)
     elif mask is not None:
         output = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, is_causal=False,
                                                 enable_gqa=enable_gqa)

@@ -244,14 +244,18 @@ class DecodeKVCache:
         self.v[bidx, :, pos] = v_new.to(self.dtype).permute(0, 2, 1, 3)
 
     def rope_append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
-                    sin: torch.Tensor, pos: torch.Tensor, q_out: torch.Tensor) -> torch.Tensor:
+                    sin: torch.Tensor, pos: torch.Tensor, q_out: torch.Tensor,
+                    q_norm: tuple | None = None, k_norm: tuple | None = None) -> torch.Tensor:
         """Rotate one decode token per sequence and append it, in one launch.
 
         q [B, 1, Hq*D], k and v [B, 1, Hkv*D] (projection outputs, heads
         contiguous), cos/sin [B, 1, D] (the model's rotary tables in its
         dtype), pos [B, 1] int64 device positions.  rope(k) and v go to the
         capacity buffers at pos; rope(q) to q_out [B, Hq, D], returned as
-        [B, Hq, 1, D].  Bit-identical to apply_rotary_pos_emb + append_at."""
+        [B, Hq, 1, D].  Bit-identical to apply_rotary_pos_emb + append_at.
+
+        q_norm, k_norm: (weight [D], eps) of an RMSNorm over each head before the
+        rotation; norm and rotation are then computed in fp32 and rounded once."""
         D, B = self.D, self.B
         Hq = q.shape[-1] // D
         if any(t.stride(-1) != 1 for t in (q, k, v, cos, sin)):
@@ -268,8 +272,67 @@ class DecodeKVCache:
             raise RuntimeError("rope_append: pos must be int64 with one position per sequence")
         if q_out.shape != (B, Hq, D) or not q_out.is_contiguous() or q_out.dtype != self.dtype:
             raise RuntimeError("rope_append: q_out must be a contiguous [B, Hq, D] tensor")
+        if q_norm is not None or k_norm is not None:
+            self._qk_rope(q, k, v, cos, sin, None, pos.reshape(B), q_norm, k_norm, q_out)
+            return q_out.unsqueeze(2)
         ops().rope_append(q, k, v, cos, sin, pos, self.k, self.v, self.capacity, q_out)
         return q_out.unsqueeze(2)
+
+    def _qk_rope(self, q, k, v, cos, sin, seq, pos, q_norm, k_norm, q_out) -> None:
+        D, n = self.D, pos.numel()
+        (qw, qe), (kw, ke) = q_norm or (None, 0.0), k_norm or (None, 0.0)
+        ops().qk_rope_append(*(x.reshape(n, -1, D) for x in (q, k, v)), cos.reshape(n, D),
+                             sin.reshape(n, D), qw, qe, kw, ke, seq, pos, self.k, self.v, q_out)
+
+    @torch.no_grad()
+    def rope_append_packed(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           cos: torch.Tensor, sin: torch.Tensor, plan,
+                           q_out: torch.Tensor | None = None, q_norm: tuple | None = None,
+                           k_norm: tuple | None = None) -> torch.Tensor:
+        """Rotate a packed pass's tokens and write them into the cache, in one launch.
+
+        q [..., n, Hq*D], k and v [..., n, Hkv*D] (projection outputs, heads
+        contiguous), cos/sin [..., n, D], plan: the pass's
+        :class:`~laprune_amd.packed.PackedPrompts` of n tokens.  rope(k) and v go to
+        their sequences' rows of the capacity buffers (tokens past the capacity are
+        not written), rope(q) to q_out [n, Hq, D], which is returned.  Norms as in
+        :meth:`rope_append`; without them bit-identical to its rotation.  Lengths are
+        the caller's (:meth:`append_packed` keeps them)."""
+        D, n = self.D, plan.total
+        if plan.B != self.B:
+            raise RuntimeError(f"rope_append_packed: a plan of {plan.B} sequences, not {self.B}")
+        if any(t.dtype != self.dtype for t in (q, k, v, cos, sin)):
+            raise RuntimeError("rope_append_packed: q, k, v, cos and sin must be in the cache dtype")
+        if (any(t.numel() != n * t.shape[-1] for t in (q, k, v, cos, sin)) or q.shape[-1] % D
+                or k.shape[-1] != self.Hkv * D or v.shape[-1] != self.Hkv * D
+                or cos.shape[-1] != D or sin.shape[-1] != D):
+            raise RuntimeError("rope_append_packed: q [n, Hq*D], k/v [n, Hkv*D], cos/sin [n, D] "
+                               f"of n = {n} tokens expected")
+        Hq = q.shape[-1] // D
+        if q_out is None:
+            q_out = q.new_empty((n, Hq, D))
+        elif q_out.shape != (n, Hq, D) or not q_out.is_contiguous() or q_out.dtype != self.dtype:
+            raise RuntimeError("rope_append_packed: q_out must be a contiguous [n, Hq, D] tensor")
+        if n:
+            self._qk_rope(q, k, v, cos, sin, plan.seq, plan.pos, q_norm, k_norm, q_out)
+        return q_out
+
+    def append_packed(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      cos: torch.Tensor, sin: torch.Tensor, plan, q_norm: tuple | None = None,
+                      k_norm: tuple | None = None) -> torch.Tensor:
+        """:meth:`rope_append_packed` behind every sequence's cached tokens, growing
+        the buffers when needed, and the encode of all new keys (a prompt's).  The
+        plan's host lengths must continue this cache's."""
+        if plan.lens is None or plan.cached != self.lengths:
+            raise RuntimeError("append_packed: the plan's cached lengths are not the cache's "
+                               f"({plan.cached}, {self.lengths})")
+        ends = [n + t for n, t in zip(plan.lens, plan.cached)]
+        if max(ends) > self.capacity:
+            self._grow(max(ends))
+        q_out = self.rope_append_packed(q, k, v, cos, sin, plan, None, q_norm, k_norm)
+        self.lengths = ends
+        self._encode_rows([b for b in range(self.B) if plan.lens[b]], True, None)
+        return q_out
 
     def encode_ranges(self, ranges: torch.Tensor) -> None:
         """Encode each sequence's device range ([B, 2] int32, at most

@@ -1,0 +1,699 @@
+// prompt.hip — attention of many query rows over a K/V cache: causal attention of
+// packed prompts (grouped heads, sequences of different lengths, tokens cached
+// before them), and a decode step over a cache whose first tokens are the same in
+// every sequence.
+//
+// Both are, per KV head, a block of rows (a row is one query head of one token) over
+// a range of keys:
+//   o[r] = sum_{t < lim[r]} 2^(c (q[r].k[t]) - m[r]) v[t] / sum of the same weights,
+// c = scale * log2(e), m the row's running maximum (one pass over the keys, fp32).
+//
+// Products are 32x32x16 MFMAs with the scores transposed, S^T = K Q^T: a lane then
+// holds 16 keys of one query (column lane % 32, keys 8 i + 4 (lane / 32) + e), so a
+// row's maximum and sum are lane-local but for one exchange with lane + 32, and the
+// weights are, in place, the B operand of o^T = V^T P^T (the reduction's order of
+// keys is free as long as V^T's operand uses the same).  V^T comes from the row-major
+// V tile through the transposing LDS read.
+//
+// All query heads of a KV head lie in one block (row = token * G + head): K and V are
+// read once for the group, and 32 rows span few tokens, so little of a causal block
+// is masked.  A wave skips a tile of keys that none of its rows sees.
+#include "common.h"
+#include "attn_core.h"
+
+#include <algorithm>
+
+namespace lap {
+namespace {
+
+constexpr int kBN = 64;  // keys per tile
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+#define LAP_LDS __attribute__((address_space(3)))
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(i16x8 a, i16x8 b, f32x16 c) {
+  if constexpr (DT == LAP_DTYPE_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Two weights in the data type, round to nearest even.  The weights enter the second
+// product in 16 bits (half a step, 2^-9 or 2^-12 of each); their sum stays fp32.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == LAP_DTYPE_F16) {
+    const f16x2 r = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, r);
+  } else {
+    const bf16x2 r = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, r);
+  }
+}
+
+// Swizzle of a tile row: the row's 16-byte chunks are stored at chunk ^ swz(row).
+// 16 rows of one chunk (a K read) then fall in 16 different slots of 256 bytes, and
+// 4 rows of 64 contiguous bytes (a V read) in four different quarters.
+template <int D>
+__device__ __forceinline__ int swz(int row) {
+  if constexpr (D == 64) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
+  return (row & 3) << 2 | ((row >> 2) & 3);
+}
+
+struct FlashArgs {
+  const uint16_t* q;
+  int64_t q_sb, q_st, q_sh;  // per sequence (uniform form), token, head
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+  int B, Hq, Hkv, G;
+  int Tq, Tk;        // query tokens (of a sequence, or packed), cache rows
+  const int4* tiles; // packed form
+  int bt;            // tokens per tile
+  int tps;           // uniform form: tiles per sequence
+  int nsplit, per_split;
+  float c;           // scale * log2(e)
+  uint16_t* out;
+  int64_t o_sb, o_st, o_sh;
+  float* part_o;     // [rows][nsplit][D]
+  float* part_ml;    // [rows][nsplit][2]
+  // decode over a shared prefix
+  int prefix;             // keys that every sequence shares, read from sequence 0
+  int psplit, pblocks;    // splits of the prefix, row blocks of it
+  const int32_t* plans;   // lap_row_plan[B] (t_total), or null: Tk keys each
+};
+
+// What a workgroup works on.
+struct FlashTile {
+  const uint16_t* q;   // token 0 of the tile, query head 0 of the KV head
+  uint16_t* out;
+  int64_t q_st, o_st;  // per token
+  int64_t row0;        // row of part_* of token 0, head 0 of the KV head
+  const uint16_t* k;   // row 0 of the sequence's keys
+  const uint16_t* v;
+  int n;               // tokens
+  int key0;            // token j sees keys [0, key0 + j + 1), or
+  const int32_t* lens; // [0, min(hi, lens[8 j])) where not null
+  int lo, hi;          // keys of this workgroup
+  int split;
+};
+
+// The tile of 64 keys from kt, rows past the last key of the range repeat it.
+template <int D, int NW>
+__device__ __forceinline__ void load_tile(char* s_dst, const uint16_t* base, int64_t st, int kt,
+                                          int last, int tid) {
+  constexpr int C = D / 8, PER = kBN * C / (64 * NW);
+  const int wave = tid >> 6, lane = tid & 63;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int slot0 = (i * NW + wave) * 64, slot = slot0 + lane;
+    const int row = slot / C, chunk = (slot % C) ^ swz<D>(row);
+    const uint16_t* g = base + (int64_t)min(kt + row, last) * st + chunk * 8;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                     (LAP_LDS void*)(s_dst + slot0 * 16), 16, 0, 0);
+  }
+}
+
+template <int DT, int D, int NW, bool SHARED>
+__device__ __forceinline__ void flash(const FlashArgs& a, const FlashTile& t, char* s_k,
+                                      char* s_v) {
+  constexpr int KS = D / 16, DC = D / 32, C = D / 8;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = lane & 31, hl = lane >> 5;
+  const int row = wave * 32 + col, j = row / a.G, head = row - j * a.G;
+  const bool live = j < t.n;
+  int lim, w_max, w_min;  // keys that this row, some row and every row of the wave sees
+  if (SHARED && t.lens) {
+    lim = live ? t.lens[j * kPlanInts + 1] : 0;
+    w_max = lim;
+    w_min = live ? lim : INT32_MAX;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+      w_max = max(w_max, __shfl_xor(w_max, d, 64));
+      w_min = min(w_min, __shfl_xor(w_min, d, 64));
+    }
+  } else {
+    lim = live ? t.key0 + j + 1 : 0;
+    const int j_lo = wave * 32 / a.G, j_hi = min((wave * 32 + 31) / a.G, t.n - 1);
+    w_max = j_lo < t.n ? t.key0 + (SHARED ? 0 : j_hi) + 1 : 0;
+    w_min = t.key0 + (SHARED ? 0 : j_lo) + 1;
+    if (SHARED) lim = live ? t.key0 + 1 : 0;  // a step's tokens do not see each other
+  }
+  w_max = __builtin_amdgcn_readfirstlane(w_max);
+  w_min = __builtin_amdgcn_readfirstlane(w_min);
+
+  i16x8 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    qf[ks] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (live)
+      qf[ks] = *reinterpret_cast<const i16x8*>(t.q + j * t.q_st + head * a.q_sh + ks * 16 + hl * 8);
+  }
+  f32x16 o[DC];
+#pragma unroll
+  for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dc][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  for (int kt = t.lo; kt < t.hi; kt += kBN) {
+    __syncthreads();
+    load_tile<D, NW>(s_k, t.k, a.k_st, kt, t.hi - 1, tid);
+    load_tile<D, NW>(s_v, t.v, a.v_st, kt, t.hi - 1, tid);
+    __syncthreads();
+    if (kt >= w_max) continue;
+    f32x16 s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
+      const int r = h * 32 + col;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const i16x8 kf = *reinterpret_cast<const i16x8*>(
+            s_k + (r * C + ((2 * ks + hl) ^ swz<D>(r))) * 16);
+        s[h] = mfma32<DT>(kf, qf[ks], s[h]);
+      }
+    }
+    const int end = min(lim, t.hi);
+    const bool masked = kt + kBN > min(w_min, t.hi);
+    if (masked) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (kt + h * 32 + (i & 3) + 8 * (i >> 2) + 4 * hl >= end) s[h][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[h][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float m_new = fmaxf(m, mx * a.c);
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], a.c, -m_use));
+        s[h][i] = p;
+        sum += p;
+      }
+    l = __builtin_fmaf(l, alpha, sum);
+    m = m_new;
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dc][i] *= alpha;
+
+    uint32_t pk[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pk[8 * h + i] = pack2<DT>(s[h][2 * i], s[h][2 * i + 1]);
+
+    // A value that is not finite in a row that some of these queries do not see must
+    // not reach them as 0 * inf: such a tile is summed key by key instead.
+    bool dirty = false;
+    if (masked) {
+      u16x2 top = {0, 0};
+      for (int i = lane; i < kBN * C; i += 64) {
+        const int r = i / C;
+        if (kt + r < w_min) continue;
+        const uint4 w = *reinterpret_cast<const uint4*>(s_v + i * 16);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+      }
+      constexpr unsigned short kInf = DT == LAP_DTYPE_F16 ? 0x7c00 : 0x7f80;
+      dirty = __ballot(top[0] >= kInf || top[1] >= kInf) != 0;
+    }
+    if (!dirty) {
+      const int g16 = (lane >> 4) & 1, i16 = lane & 15;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const uint4 pw = make_uint4(pk[4 * ks], pk[4 * ks + 1], pk[4 * ks + 2], pk[4 * ks + 3]);
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) {
+          i16x4 vt[2];
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const int r = 16 * ks + 8 * jj + 4 * hl + (i16 >> 2);
+            const int chunk = 4 * dc + 2 * g16 + ((i16 & 3) >> 1);
+            vt[jj] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (LAP_LDS i16x4*)(s_v + (r * C + (chunk ^ swz<D>(r))) * 16 + (i16 & 1) * 8));
+          }
+          const i16x8 vf = {vt[0][0], vt[0][1], vt[0][2], vt[0][3],
+                            vt[1][0], vt[1][1], vt[1][2], vt[1][3]};
+          o[dc] = mfma32<DT>(vf, __builtin_bit_cast(i16x8, pw), o[dc]);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int r = 0; r < kBN && kt + r < t.hi; ++r) {
+        // the weight of key r: register 4 * (r / 8) + r % 4 of half r / 32, in the lane
+        // of the pair with hl = r / 4 % 2
+        const int want = (r >> 5) * 8 + ((r >> 3) & 3) * 2 + ((r & 3) >> 1);
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w = i == want ? pk[i] : w;
+        w = __shfl(w, col + 32 * ((r >> 2) & 1), 64);
+        const float p = ld16<DT>((uint16_t)(r & 1 ? w >> 16 : w));
+        const bool sees = kt + r < end;
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int d = 32 * dc + (i & 3) + 8 * (i >> 2) + 4 * hl;
+            const float x = ld16<DT>(*reinterpret_cast<const uint16_t*>(
+                s_v + (r * C + ((d >> 3) ^ swz<D>(r))) * 16 + (d & 7) * 2));
+            o[dc][i] = sees ? __builtin_fmaf(p, x, o[dc][i]) : o[dc][i];
+          }
+      }
+    }
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (!live) return;
+  if (a.nsplit == 1) {
+    // weights that sum to zero (no key, or all scores -inf) give zeros
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t* op = t.out + j * t.o_st + head * a.o_sh;
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint2 w;
+        w.x = pack2<DT>(o[dc][4 * g] * inv, o[dc][4 * g + 1] * inv);
+        w.y = pack2<DT>(o[dc][4 * g + 2] * inv, o[dc][4 * g + 3] * inv);
+        *reinterpret_cast<uint2*>(op + 32 * dc + 8 * g + 4 * hl) = w;
+      }
+    return;
+  }
+  const int64_t at = (t.row0 + (int64_t)j * a.Hq + head) * a.nsplit + t.split;
+  if (hl == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+#pragma unroll
+  for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(a.part_o + at * D + 32 * dc + 8 * g + 4 * hl) =
+          make_float4(o[dc][4 * g], o[dc][4 * g + 1], o[dc][4 * g + 2], o[dc][4 * g + 3]);
+}
+
+// Tile ti of a prompt call: its sequence, first token (of the sequence in the uniform
+// form, of all in the packed one), tokens and cached keys; false: nothing to do.
+struct PromptTile {
+  int b, q0, n, key0;
+};
+__device__ __forceinline__ bool prompt_tile(const FlashArgs& a, int ti, PromptTile& p) {
+  if (a.tiles) {
+    const int4 w = a.tiles[ti];
+    p = {w.z, w.x, min(min(w.y, a.bt), a.Tq - w.x), w.w};
+    return p.n > 0 && p.q0 >= 0 && p.b >= 0 && p.b < a.B && p.key0 >= 0;
+  }
+  // B sequences of Tq tokens at the end of Tk keys, the last tokens first
+  const int i = a.tps - 1 - ti / a.B;
+  p = {ti % a.B, i * a.bt, min(a.bt, a.Tq - i * a.bt), a.Tk - a.Tq + i * a.bt};
+  return true;
+}
+__device__ __forceinline__ int64_t prompt_row(const FlashArgs& a, const PromptTile& p) {
+  return (a.tiles ? 0 : (int64_t)p.b * a.Tq) + p.q0;
+}
+
+// Workgroup -> (tile, split, KV head), the KV head fastest: consecutive workgroups go
+// to different XCDs, so an XCD's L2 holds the keys of few heads.
+template <int DT, int D, int NW>
+__global__ __launch_bounds__(64 * NW) void prompt_kernel(FlashArgs a) {
+  __shared__ __attribute__((aligned(256))) char s_k[kBN * D * 2], s_v[kBN * D * 2];
+  const int hkv = blockIdx.x % a.Hkv;
+  const int rest = blockIdx.x / a.Hkv;
+  const int split = rest % a.nsplit;
+  PromptTile p;
+  if (!prompt_tile(a, rest / a.nsplit, p)) return;
+  const int64_t qb = a.tiles ? 0 : p.b;
+  FlashTile t;
+  t.n = p.n;
+  t.key0 = p.key0;
+  t.lens = nullptr;
+  t.row0 = prompt_row(a, p) * a.Hq + hkv * a.G;
+  t.q = a.q + qb * a.q_sb + (int64_t)p.q0 * a.q_st + (int64_t)hkv * a.G * a.q_sh;
+  t.out = a.out + qb * a.o_sb + (int64_t)p.q0 * a.o_st + (int64_t)hkv * a.G * a.o_sh;
+  t.q_st = a.q_st;
+  t.o_st = a.o_st;
+  t.k = a.k + (int64_t)p.b * a.k_sb + (int64_t)hkv * a.k_sh;
+  t.v = a.v + (int64_t)p.b * a.v_sb + (int64_t)hkv * a.v_sh;
+  // the last split takes what is left; no key past the cache is read
+  const int keys = min(p.key0 + p.n, a.Tk);
+  t.split = split;
+  t.lo = (int)min((int64_t)split * a.per_split, (int64_t)keys);
+  t.hi = split == a.nsplit - 1 ? keys : min(keys, t.lo + a.per_split);
+  flash<DT, D, NW, false>(a, t, s_k, s_v);
+}
+
+// One query token per sequence over keys of which the first `prefix` are the same in
+// every sequence.  Items: for the prefix, blocks of as many sequences as fill the
+// workgroup's rows, by splits of the keys of sequence 0; behind it, each sequence by
+// splits of its own keys.
+template <int DT, int D, int NW>
+__global__ __launch_bounds__(64 * NW) void shared_kernel(FlashArgs a) {
+  __shared__ __attribute__((aligned(256))) char s_k[kBN * D * 2], s_v[kBN * D * 2];
+  const int hkv = blockIdx.x % a.Hkv;
+  const int it = blockIdx.x / a.Hkv, n_pre = a.psplit * a.pblocks;
+  FlashTile t;
+  int b, kb = 0;
+  if (it < n_pre) {
+    b = it / a.psplit * a.bt;
+    t.split = it % a.psplit;
+    t.n = min(a.bt, a.B - b);
+    t.key0 = a.Tk - 1;
+    t.lens = a.plans ? a.plans + (int64_t)b * kPlanInts : nullptr;
+    t.lo = t.split * a.per_split;
+    t.hi = min(a.prefix, t.lo + a.per_split);
+  } else {
+    const int ss = a.nsplit - a.psplit, i = (it - n_pre) % ss;
+    b = kb = (it - n_pre) / ss;
+    t.split = a.psplit + i;
+    t.n = 1;
+    const int len = a.plans ? min(a.plans[(int64_t)b * kPlanInts + 1], a.Tk) : a.Tk;
+    t.key0 = len - 1;
+    t.lens = nullptr;
+    t.lo = (int)min((int64_t)a.prefix + (int64_t)i * a.per_split, (int64_t)a.Tk);
+    t.hi = min(len, t.lo + a.per_split);
+  }
+  t.row0 = (int64_t)b * a.Hq + hkv * a.G;
+  t.q = a.q + (int64_t)b * a.q_sb + (int64_t)hkv * a.G * a.q_sh;
+  t.out = a.out + t.row0 * D;
+  t.q_st = a.q_sb;
+  t.o_st = (int64_t)a.Hq * D;
+  t.k = a.k + (int64_t)kb * a.k_sb + (int64_t)hkv * a.k_sh;
+  t.v = a.v + (int64_t)kb * a.v_sb + (int64_t)hkv * a.v_sh;
+  flash<DT, D, NW, true>(a, t, s_k, s_v);
+}
+
+// out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) of one row: four waves take the
+// splits in turn, a lane D / 64 of the row's values.
+template <int DT, int D>
+__device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, uint16_t* out) {
+  constexpr int V = D / 64;
+  __shared__ float s_o[4][D], s_l[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float* ml = a.part_ml + row * a.nsplit * 2;
+  float M = -INFINITY;
+  for (int s = lane; s < a.nsplit; s += 64) M = fmaxf(M, ml[2 * s]);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  const float base = M == -INFINITY ? 0.f : M;
+  float o[V] = {}, l = 0.f;
+  const float* po = a.part_o + row * a.nsplit * D + lane * V;
+  for (int s = wave; s < a.nsplit; s += 4) {
+    const float ls = ml[2 * s + 1];
+    if (ls == 0.f) continue;  // nothing of this row in the split
+    const float w = __builtin_amdgcn_exp2f(ml[2 * s] - base);
+    l = __builtin_fmaf(ls, w, l);
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(po[(int64_t)s * D + e], w, o[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) s_o[wave][lane * V + e] = o[e];
+  if (lane == 0) s_l[wave] = l;
+  __syncthreads();
+  if (tid >= D) return;
+  const float all = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+  const float x = s_o[0][tid] + s_o[1][tid] + s_o[2][tid] + s_o[3][tid];
+  out[tid] = st16<DT>(all == 0.f ? 0.f : x / all);
+}
+
+// One workgroup per (tile, token, head); only rows of a tile are written.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void prompt_merge_kernel(FlashArgs a) {
+  const int h = blockIdx.x % a.Hq, rest = blockIdx.x / a.Hq;
+  const int j = rest % a.bt;
+  PromptTile p;
+  if (!prompt_tile(a, rest / a.bt, p) || j >= p.n) return;
+  uint16_t* out = a.out + (a.tiles ? 0 : p.b) * a.o_sb + (int64_t)(p.q0 + j) * a.o_st + h * a.o_sh;
+  merge_row<DT, D>(a, (prompt_row(a, p) + j) * a.Hq + h, out);
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(256) void shared_merge_kernel(FlashArgs a) {
+  merge_row<DT, D>(a, blockIdx.x, a.out + (int64_t)blockIdx.x * D);
+}
+
+#define LAP_BY_NW(KERNEL)                                                              \
+  do {                                                                                \
+    if (nw == 1) hipLaunchKernelGGL((KERNEL<DT, D, 1>), g, dim3(64), 0, st, a);       \
+    else if (nw == 2) hipLaunchKernelGGL((KERNEL<DT, D, 2>), g, dim3(128), 0, st, a); \
+    else if (nw == 4) hipLaunchKernelGGL((KERNEL<DT, D, 4>), g, dim3(256), 0, st, a); \
+    else hipLaunchKernelGGL((KERNEL<DT, D, 8>), g, dim3(512), 0, st, a);              \
+  } while (0)
+
+// The kernel and, with more than one split, the merge.
+template <bool SHARED, int DT, int D>
+int launch_flash(const FlashArgs& a, int nw, int64_t grid, int64_t merge_grid, hipStream_t st) {
+  const dim3 g((unsigned)grid), mg((unsigned)merge_grid);
+  if constexpr (SHARED) LAP_BY_NW(shared_kernel);
+  else LAP_BY_NW(prompt_kernel);
+  LAP_LAUNCH_CHECK("attention of many rows");
+  if (a.nsplit > 1) {
+    if constexpr (SHARED) hipLaunchKernelGGL((shared_merge_kernel<DT, D>), mg, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((prompt_merge_kernel<DT, D>), mg, dim3(256), 0, st, a);
+    LAP_LAUNCH_CHECK("merge of splits");
+  }
+  return LAP_OK;
+}
+#undef LAP_BY_NW
+
+template <bool SHARED>
+int launch_by_type(const FlashArgs& a, int dtype, int D, int nw, int64_t grid, int64_t merge_grid,
+                   hipStream_t st) {
+#define LAP_BY_D(DT)                                                             \
+  return D == 64    ? launch_flash<SHARED, DT, 64>(a, nw, grid, merge_grid, st)  \
+         : D == 128 ? launch_flash<SHARED, DT, 128>(a, nw, grid, merge_grid, st) \
+                    : launch_flash<SHARED, DT, 256>(a, nw, grid, merge_grid, st)
+  if (dtype == LAP_DTYPE_F16) LAP_BY_D(LAP_DTYPE_F16);
+  LAP_BY_D(LAP_DTYPE_BF16);
+#undef LAP_BY_D
+}
+
+int waves_of(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }
+
+size_t part_bytes(int64_t rows, int nsplit, int D) {
+  return nsplit > 1 ? (size_t)rows * nsplit * (D + 2) * sizeof(float) : 0;
+}
+
+int check_heads(const char* fn, int Hq, int Hkv, int D) {
+  LAP_CHECK(Hq > 0 && Hkv > 0 && D > 0, "%s: bad sizes", fn);
+  LAP_CHECK(Hq % Hkv == 0, "invalid GQA head counts: Hq=%d, Hkv=%d", Hq, Hkv);
+  LAP_CHECK_CODE(Hq / Hkv <= 256, LAP_ERR_UNSUPPORTED, "%s: group size %d unsupported (1 to 256)",
+                 fn, Hq / Hkv);
+  LAP_CHECK_CODE(D == 64 || D == 128 || D == 256, LAP_ERR_UNSUPPORTED,
+                 "%s: head dim %d unsupported (64/128/256)", fn, D);
+  return LAP_OK;
+}
+
+}  // namespace
+}  // namespace lap
+
+using namespace lap;
+
+extern "C" int lap_prompt_shape(int total, int B, int max_keys, int Hq, int Hkv, int D,
+                                int* tokens_per_tile, int* n_tiles, int* nsplit) {
+  clear_error();
+  LAP_CHECK(tokens_per_tile && n_tiles && nsplit, "lap_prompt_shape: null output");
+  LAP_CHECK(total >= 0 && B > 0 && max_keys >= 0, "lap_prompt_shape: bad sizes");
+  int s = check_heads("lap_prompt_shape", Hq, Hkv, D);
+  if (s != LAP_OK) return s;
+  constexpr int kCUs = 256;
+  const int G = Hq / Hkv;
+  int nw = 8;
+  auto tiles_of = [&](int w) { return (int64_t)total / (32 * w / G) + std::min(B, total); };
+  while (nw > 1 && 32 * (nw / 2) >= G && tiles_of(nw) * Hkv < 2 * kCUs) nw /= 2;
+  const int64_t items = tiles_of(nw) * Hkv;
+  int ns = 1;
+  if (items < 2 * kCUs && items > 0) {
+    ns = (int)std::min<int64_t>(2 * kCUs / items, ((int64_t)max_keys + 255) / 256);
+    ns = std::max(1, std::min(ns, 256));
+  }
+  *tokens_per_tile = 32 * nw / G;
+  *n_tiles = (int)tiles_of(nw);
+  *nsplit = ns;
+  return LAP_OK;
+}
+
+extern "C" int lap_prompt_attention_workspace_size(int64_t tokens, int Hq, int D, int nsplit,
+                                                   size_t* bytes) {
+  clear_error();
+  LAP_CHECK(bytes, "lap_prompt_attention_workspace_size: null output");
+  LAP_CHECK(tokens >= 0 && Hq > 0 && D > 0 && nsplit > 0, "bad sizes");
+  *bytes = part_bytes(tokens * Hq, nsplit, D);
+  return LAP_OK;
+}
+
+extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                    const void* keys, const void* vals, int64_t k_sb, int64_t k_sh,
+                                    int64_t k_st, int64_t v_sb, int64_t v_sh, int64_t v_st,
+                                    int dtype, int B, int Hq, int Hkv, int D, int Tq, int Tk,
+                                    const int32_t* tiles, int n_tiles, int tokens_per_tile,
+                                    int nsplit, int max_keys, float scale, void* out, int64_t o_sb,
+                                    int64_t o_st, int64_t o_sh, void* workspace,
+                                    size_t workspace_bytes, lap_stream_t stream) {
+  clear_error();
+  LAP_CHECK(q && keys && vals && out, "lap_prompt_attention: null pointer");
+  LAP_CHECK(dtype == LAP_DTYPE_F16 || dtype == LAP_DTYPE_BF16,
+            "lap_prompt_attention: dtype must be fp16/bf16");
+  LAP_CHECK(B > 0 && Tq > 0 && Tk > 0 && Tk < (1 << 30), "lap_prompt_attention: bad sizes");
+  int s = check_heads("lap_prompt_attention", Hq, Hkv, D);
+  if (s != LAP_OK) return s;
+  LAP_CHECK(tiles || Tq <= Tk, "lap_prompt_attention: %d queries exceed %d keys", Tq, Tk);
+  LAP_CHECK(scale > 0.f && scale < INFINITY, "lap_prompt_attention: scale must be positive");
+  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(keys) |
+                         reinterpret_cast<uintptr_t>(vals) | reinterpret_cast<uintptr_t>(out) |
+                         reinterpret_cast<uintptr_t>(tiles);
+  LAP_CHECK((ptrs & 15) == 0 && ((q_sb | q_st | q_sh | k_sb | k_sh | k_st | v_sb | v_sh | v_st |
+                                  o_sb | o_st | o_sh) & 7) == 0,
+            "lap_prompt_attention: rows must be 16-byte aligned");
+  const int G = Hq / Hkv;
+  LAP_CHECK(tokens_per_tile > 0 && (int64_t)tokens_per_tile * G <= 256 && nsplit > 0 &&
+                n_tiles >= 0 && max_keys >= 0,
+            "lap_prompt_attention: bad tile shape");
+  if (!tiles) n_tiles = B * ((Tq + tokens_per_tile - 1) / tokens_per_tile);
+  if (n_tiles == 0) return LAP_OK;
+  FlashArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
+  a.k = static_cast<const uint16_t*>(keys);
+  a.v = static_cast<const uint16_t*>(vals);
+  a.k_sb = k_sb; a.k_sh = k_sh; a.k_st = k_st;
+  a.v_sb = v_sb; a.v_sh = v_sh; a.v_st = v_st;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = G; a.Tq = Tq; a.Tk = Tk;
+  a.tiles = reinterpret_cast<const int4*>(tiles);
+  a.bt = tokens_per_tile;
+  a.tps = (Tq + tokens_per_tile - 1) / tokens_per_tile;
+  a.nsplit = nsplit;
+  a.per_split = (std::max(1, (std::min(max_keys, Tk) + nsplit - 1) / nsplit) + kBN - 1) / kBN * kBN;
+  a.c = scale * kLog2e;
+  a.out = static_cast<uint16_t*>(out);
+  a.o_sb = o_sb; a.o_st = o_st; a.o_sh = o_sh;
+  const int64_t rows = (int64_t)(tiles ? 1 : B) * Tq * Hq;
+  const int64_t grid = (int64_t)n_tiles * nsplit * Hkv;
+  LAP_CHECK(grid <= 0x7fffffff && (int64_t)n_tiles * tokens_per_tile * Hq <= 0x7fffffff,
+            "lap_prompt_attention: too many rows");
+  if (nsplit > 1) {
+    const size_t need = part_bytes(rows, nsplit, D);
+    LAP_CHECK_CODE(workspace && workspace_bytes >= need, LAP_ERR_WORKSPACE,
+                   "lap_prompt_attention: workspace of %zu bytes needed", need);
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + rows * nsplit * D;
+  }
+  return launch_by_type<false>(a, dtype, D, waves_of(tokens_per_tile * G), grid,
+                               (int64_t)n_tiles * tokens_per_tile * Hq, as_stream(stream));
+}
+
+namespace lap {
+namespace {
+
+// Rows per block, keys per split and splits of a decode step over a shared prefix.
+struct SharedShape {
+  int nw, bt, pblocks, per, psplit, nsplit;
+};
+SharedShape shared_shape(int B, int Hkv, int G, int T, int prefix) {
+  constexpr int kItems = 1024;
+  SharedShape s;
+  s.nw = waves_of((int)std::min<int64_t>((int64_t)B * G, 256));
+  while (32 * s.nw < G) s.nw *= 2;
+  s.bt = 32 * s.nw / G;
+  s.pblocks = (B + s.bt - 1) / s.bt;
+  const int64_t keys = ((int64_t)s.pblocks * prefix + (int64_t)B * (T - prefix)) * Hkv;
+  int64_t per = std::max<int64_t>({128, (keys + kItems - 1) / kItems, (T + 511) / 512});
+  s.per = (int)((per + kBN - 1) / kBN * kBN);
+  s.psplit = (prefix + s.per - 1) / s.per;
+  s.nsplit = s.psplit + (T - prefix + s.per - 1) / s.per;
+  return s;
+}
+
+int check_shared(int B, int Hq, int Hkv, int D, int T, int prefix) {
+  LAP_CHECK(B > 0 && T > 0 && T < (1 << 30), "shared-prefix decode: bad sizes");
+  int s = check_heads("shared-prefix decode", Hq, Hkv, D);
+  if (s != LAP_OK) return s;
+  LAP_CHECK(prefix >= 0 && prefix <= T, "shared-prefix decode: a prefix of %d of %d keys", prefix, T);
+  return LAP_OK;
+}
+
+}  // namespace
+}  // namespace lap
+
+extern "C" int lap_shared_attn_decode_workspace_size(int B, int Hq, int Hkv, int D, int T,
+                                                     int prefix, size_t* bytes) {
+  clear_error();
+  LAP_CHECK(bytes, "lap_shared_attn_decode_workspace_size: null output");
+  int s = check_shared(B, Hq, Hkv, D, T, prefix);
+  if (s != LAP_OK) return s;
+  *bytes = part_bytes((int64_t)B * Hq, shared_shape(B, Hkv, Hq / Hkv, T, prefix).nsplit, D);
+  return LAP_OK;
+}
+
+extern "C" int lap_shared_attn_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* keys,
+                                      const void* vals, int dtype, int B, int Hq, int Hkv, int T,
+                                      int D, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                                      int64_t v_sb, int64_t v_sh, int64_t v_st, int prefix,
+                                      const lap_row_plan* plans, float scale, void* out,
+                                      void* workspace, size_t workspace_bytes,
+                                      lap_stream_t stream) {
+  clear_error();
+  LAP_CHECK(q && keys && vals && out, "lap_shared_attn_decode: null pointer");
+  LAP_CHECK(dtype == LAP_DTYPE_F16 || dtype == LAP_DTYPE_BF16,
+            "lap_shared_attn_decode: dtype must be fp16/bf16");
+  int s = check_shared(B, Hq, Hkv, D, T, prefix);
+  if (s != LAP_OK) return s;
+  LAP_CHECK(scale > 0.f && scale < INFINITY, "lap_shared_attn_decode: scale must be positive");
+  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(keys) |
+                         reinterpret_cast<uintptr_t>(vals) | reinterpret_cast<uintptr_t>(out);
+  LAP_CHECK((ptrs & 15) == 0 &&
+                ((q_sb | q_sh | k_sb | k_sh | k_st | v_sb | v_sh | v_st) & 7) == 0,
+            "lap_shared_attn_decode: rows must be 16-byte aligned");
+  const SharedShape sh = shared_shape(B, Hkv, Hq / Hkv, T, prefix);
+  FlashArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_sb = q_sb; a.q_sh = q_sh;
+  a.k = static_cast<const uint16_t*>(keys);
+  a.v = static_cast<const uint16_t*>(vals);
+  a.k_sb = k_sb; a.k_sh = k_sh; a.k_st = k_st;
+  a.v_sb = v_sb; a.v_sh = v_sh; a.v_st = v_st;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.Tq = 1; a.Tk = T;
+  a.bt = sh.bt;
+  a.nsplit = sh.nsplit;
+  a.per_split = sh.per;
+  a.c = scale * kLog2e;
+  a.out = static_cast<uint16_t*>(out);
+  a.o_sh = D;
+  a.prefix = prefix;
+  a.psplit = sh.psplit;
+  a.pblocks = sh.pblocks;
+  a.plans = reinterpret_cast<const int32_t*>(plans);
+  const int64_t rows = (int64_t)B * Hq;
+  const int64_t grid =
+      ((int64_t)sh.pblocks * sh.psplit + (int64_t)B * (sh.nsplit - sh.psplit)) * Hkv;
+  LAP_CHECK(grid <= 0x7fffffff && rows <= 0x7fffffff, "lap_shared_attn_decode: too many rows");
+  if (sh.nsplit > 1) {
+    const size_t need = part_bytes(rows, sh.nsplit, D);
+    LAP_CHECK_CODE(workspace && workspace_bytes >= need, LAP_ERR_WORKSPACE,
+                   "lap_shared_attn_decode: workspace of %zu bytes needed", need);
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + rows * sh.nsplit * D;
+  }
+  return launch_by_type<true>(a, dtype, D, sh.nw, grid, rows, as_stream(stream));
+}

@@ -12,6 +12,7 @@
 // built with hipcc against the torch headers, linked to the HIP library.
 #include <torch/library.h>
 #include <ATen/core/Tensor.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -332,6 +333,153 @@ void argmax_rows(const at::Tensor& x, const at::Tensor& out,
         "lap_argmax_rows");
 }
 
+// Packed prompts and decode over a shared prefix (csrc/pack.hip, csrc/cache.hip,
+// csrc/prompt.hip).  The calls run on the tensors' device, current or not.
+void pack_prompts(const at::Tensor& new_lens, const std::optional<at::Tensor>& cached,
+                  int64_t total, int64_t tokens_per_tile, const at::Tensor& starts,
+                  const at::Tensor& seq, const at::Tensor& pos,
+                  const std::optional<at::Tensor>& tiles) {
+  same_gpu("laprune::pack_prompts", {&new_lens, opt(cached), &starts, &seq, &pos, opt(tiles)});
+  const int64_t B = new_lens.numel();
+  TORCH_CHECK(new_lens.scalar_type() == at::kInt && new_lens.dim() == 1 &&
+                  new_lens.is_contiguous() &&
+                  (!cached || (cached->scalar_type() == at::kInt && cached->is_contiguous() &&
+                               cached->dim() == 1 && cached->numel() == B)),
+              "laprune::pack_prompts: int32 lengths [B]");
+  TORCH_CHECK(starts.scalar_type() == at::kInt && starts.is_contiguous() &&
+                  starts.numel() == B + 1 && seq.scalar_type() == at::kInt &&
+                  seq.is_contiguous() && seq.numel() == total && pos.scalar_type() == at::kLong &&
+                  pos.is_contiguous() && pos.numel() == total && B <= INT32_MAX &&
+                  total <= INT32_MAX &&
+                  (!tiles || (tiles->scalar_type() == at::kInt && tiles->is_contiguous() &&
+                              tiles->dim() == 2 && tiles->size(1) == 4)),
+              "laprune::pack_prompts: starts int32 [B + 1], seq int32 and pos int64 [total], "
+              "tiles int32 [n, 4]");
+  const c10::DeviceGuard guard(starts.device());
+  check(lap_pack_prompts(static_cast<const int32_t*>(ptr(new_lens)),
+                         static_cast<const int32_t*>(ptr(cached)), (int)B, (int)total,
+                         (int)tokens_per_tile, tiles ? (int)tiles->size(0) : 0,
+                         static_cast<int32_t*>(ptr(starts)), static_cast<int32_t*>(ptr(seq)),
+                         static_cast<int64_t*>(ptr(pos)), static_cast<int32_t*>(ptr(tiles)),
+                         stream_of(starts)),
+        "lap_pack_prompts");
+}
+
+// q [n, Hq, D], k / v [n, Hkv, D], cos / sin [n, D] or [1, D], caches [B, Hkv, T, D].
+void qk_rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                    const at::Tensor& cos, const at::Tensor& sin,
+                    const std::optional<at::Tensor>& q_weight, double q_eps,
+                    const std::optional<at::Tensor>& k_weight, double k_eps,
+                    const std::optional<at::Tensor>& seq, const at::Tensor& pos,
+                    const at::Tensor& cache_k, const at::Tensor& cache_v,
+                    const at::Tensor& q_out) {
+  same_gpu("laprune::qk_rope_append", {&q, &k, &v, &cos, &sin, opt(q_weight), opt(k_weight),
+                                       opt(seq), &pos, &cache_k, &cache_v, &q_out});
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && cos.dim() == 2 && sin.dim() == 2 &&
+                  cache_k.dim() == 4 && cache_v.dim() == 4,
+              "laprune::qk_rope_append: q [n, Hq, D], k / v [n, Hkv, D], cos / sin [n, D], "
+              "caches [B, Hkv, T, D]");
+  const int64_t n = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
+  const auto dt = q.scalar_type();
+  for (const at::Tensor* t : {&q, &k, &v, &cos, &sin, &cache_k, &cache_v, &q_out})
+    TORCH_CHECK(t->scalar_type() == dt && t->size(-1) == D && t->stride(-1) == 1,
+                "laprune::qk_rope_append: one dtype, contiguous rows of head dim ", D);
+  TORCH_CHECK(k.size(0) == n && v.size(0) == n && v.size(1) == Hkv && cos.size(0) == n &&
+                  sin.size(0) == n && (n < 2 || sin.stride(0) == cos.stride(0)) &&
+                  q_out.is_contiguous() && q_out.numel() == n * Hq * D,
+              "laprune::qk_rope_append: one row of q, k, v, cos, sin and q_out per token");
+  TORCH_CHECK(cache_k.size(1) == Hkv && cache_v.sizes() == cache_k.sizes() &&
+                  cache_k.size(2) <= INT32_MAX,
+              "laprune::qk_rope_append: caches [B, Hkv, T, D] of one shape");
+  TORCH_CHECK(pos.scalar_type() == at::kLong && pos.is_contiguous() && pos.numel() == n &&
+                  (seq ? seq->scalar_type() == at::kInt && seq->is_contiguous() &&
+                             seq->numel() == n
+                       : n <= cache_k.size(0)),
+              "laprune::qk_rope_append: int64 positions and int32 sequences, one per token");
+  for (const at::Tensor* w : {opt(q_weight), opt(k_weight)})
+    TORCH_CHECK(!w || (w->scalar_type() == dt && w->is_contiguous() && w->numel() == D),
+                "laprune::qk_rope_append: norm weights [D] of the tensors' dtype");
+  const c10::DeviceGuard guard(q.device());
+  check(lap_qk_rope_append(ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1),
+                           ptr(v), v.stride(0), v.stride(1), ptr(cos), ptr(sin),
+                           n < 2 ? 0 : cos.stride(0), ptr(q_weight), (float)q_eps, ptr(k_weight),
+                           (float)k_eps, dtype_code(q), n, (int)cache_k.size(0), (int)Hq,
+                           (int)Hkv, (int)D, static_cast<const int32_t*>(ptr(seq)),
+                           static_cast<const int64_t*>(ptr(pos)), ptr(cache_k),
+                           cache_k.stride(0), cache_k.stride(1), cache_k.stride(2), ptr(cache_v),
+                           cache_v.stride(0), cache_v.stride(1), cache_v.stride(2),
+                           (int)cache_k.size(2), ptr(q_out), stream_of(q)),
+        "lap_qk_rope_append");
+}
+
+// K/V [B, Hkv, T, D] of q's dtype, head dim and device.
+void check_cache(const char* op, const at::Tensor& q, const at::Tensor& keys,
+                 const at::Tensor& vals) {
+  TORCH_CHECK(keys.dim() == 4 && vals.sizes() == keys.sizes() && keys.size(3) == q.size(-1) &&
+                  keys.scalar_type() == q.scalar_type() &&
+                  vals.scalar_type() == q.scalar_type() && keys.size(2) <= INT32_MAX,
+              op, ": keys / vals must be [B, Hkv, T, D] of q's dtype and D");
+  for (const at::Tensor* t : {&q, &keys, &vals})
+    TORCH_CHECK(t->stride(-1) == 1, op, ": rows must be contiguous");
+}
+
+// tiles given: q, out [n, Hq, D] packed; none: q, out [B, Tq, Hq, D].
+void prompt_attention(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& vals,
+                      const std::optional<at::Tensor>& tiles, int64_t tokens_per_tile,
+                      int64_t nsplit, int64_t max_keys, double scale, const at::Tensor& out,
+                      const std::optional<at::Tensor>& ws) {
+  same_gpu("laprune::prompt_attention", {&q, &keys, &vals, opt(tiles), &out, opt(ws)});
+  TORCH_CHECK(q.dim() == (tiles ? 3 : 4),
+              "laprune::prompt_attention: q [n, Hq, D] with tiles, [B, Tq, Hq, D] without");
+  check_cache("laprune::prompt_attention", q, keys, vals);
+  TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() &&
+                  out.stride(-1) == 1 && (tiles || q.size(0) == keys.size(0)),
+              "laprune::prompt_attention: out like q, as many sequences as keys");
+  TORCH_CHECK(!tiles || (tiles->scalar_type() == at::kInt && tiles->is_contiguous() &&
+                         tiles->dim() == 2 && tiles->size(1) == 4 && tiles->size(0) <= INT32_MAX),
+              "laprune::prompt_attention: tiles int32 [n, 4]");
+  TORCH_CHECK(!ws || ws->is_contiguous(), "laprune::prompt_attention: contiguous workspace");
+  const int t = tiles ? 0 : 1;  // the token dimension
+  TORCH_CHECK(q.size(t) <= INT32_MAX, "laprune::prompt_attention: too many tokens");
+  const c10::DeviceGuard guard(q.device());
+  check(lap_prompt_attention(
+            ptr(q), tiles ? 0 : q.stride(0), q.stride(t), q.stride(t + 1), ptr(keys), ptr(vals),
+            keys.stride(0), keys.stride(1), keys.stride(2), vals.stride(0), vals.stride(1),
+            vals.stride(2), dtype_code(q), (int)keys.size(0), (int)q.size(t + 1),
+            (int)keys.size(1), (int)q.size(-1), (int)q.size(t), (int)keys.size(2),
+            static_cast<const int32_t*>(ptr(tiles)), tiles ? (int)tiles->size(0) : 0,
+            (int)tokens_per_tile, (int)nsplit, (int)max_keys, (float)scale, ptr(out),
+            tiles ? 0 : out.stride(0), out.stride(t), out.stride(t + 1), ptr(ws),
+            ws ? (size_t)ws->numel() * ws->element_size() : 0, stream_of(q)),
+        "lap_prompt_attention");
+}
+
+void shared_decode(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& vals,
+                   int64_t prefix, const std::optional<at::Tensor>& plans, double scale,
+                   const at::Tensor& out, const std::optional<at::Tensor>& ws) {
+  same_gpu("laprune::shared_decode", {&q, &keys, &vals, opt(plans), &out, opt(ws)});
+  TORCH_CHECK(q.dim() == 3, "laprune::shared_decode: q [B, Hq, D]");
+  check_cache("laprune::shared_decode", q, keys, vals);
+  TORCH_CHECK(keys.size(0) == q.size(0) && out.is_contiguous() &&
+                  out.scalar_type() == q.scalar_type() && out.numel() >= q.numel(),
+              "laprune::shared_decode: as many sequences as keys, out like q");
+  TORCH_CHECK(!plans || (plans->scalar_type() == at::kInt && plans->is_contiguous() &&
+                         plans->numel() >= q.size(0) * 8),
+              "laprune::shared_decode: plans must hold B lap_row_plan records");
+  TORCH_CHECK(!ws || ws->is_contiguous(), "laprune::shared_decode: contiguous workspace");
+  TORCH_CHECK(prefix >= 0 && prefix <= keys.size(2),
+              "laprune::shared_decode: the prefix exceeds the keys");
+  const c10::DeviceGuard guard(q.device());
+  check(lap_shared_attn_decode(ptr(q), q.stride(0), q.stride(1), ptr(keys), ptr(vals),
+                               dtype_code(q), (int)q.size(0), (int)q.size(1), (int)keys.size(1),
+                               (int)keys.size(2), (int)q.size(2), keys.stride(0), keys.stride(1),
+                               keys.stride(2), vals.stride(0), vals.stride(1), vals.stride(2),
+                               (int)prefix, static_cast<const lap_row_plan*>(ptr(plans)),
+                               (float)scale, ptr(out), ptr(ws),
+                               ws ? (size_t)ws->numel() * ws->element_size() : 0, stream_of(q)),
+        "lap_shared_attn_decode");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(laprune, m) {
@@ -357,6 +505,16 @@ TORCH_LIBRARY(laprune, m) {
   m.def("silu_mul(Tensor gate, Tensor up, Tensor(a!) out) -> ()");
   m.def("rope_tables(Tensor pos, Tensor inv_freq, float scaling, Tensor(a!) cos, "
         "Tensor(b!) sin) -> ()");
+  m.def("pack_prompts(Tensor new_lens, Tensor? cached, int total, int tokens_per_tile, "
+        "Tensor(a!) starts, Tensor(b!) seq, Tensor(c!) pos, Tensor(d!)? tiles) -> ()");
+  m.def("qk_rope_append(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor? q_weight, "
+        "float q_eps, Tensor? k_weight, float k_eps, Tensor? seq, Tensor pos, "
+        "Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor(c!) q_out) -> ()");
+  m.def("prompt_attention(Tensor q, Tensor keys, Tensor vals, Tensor? tiles, "
+        "int tokens_per_tile, int nsplit, int max_keys, float scale, Tensor(a!) out, "
+        "Tensor(b!)? ws) -> ()");
+  m.def("shared_decode(Tensor q, Tensor keys, Tensor vals, int prefix, Tensor? plans, "
+        "float scale, Tensor(a!) out, Tensor(b!)? ws) -> ()");
   m.def("argmax_rows(Tensor x, Tensor(a!) out, Tensor(b!)? copy=None) -> ()");
 }
 
@@ -373,5 +531,9 @@ TORCH_LIBRARY_IMPL(laprune, CUDA, m) {
   m.impl("gemv_glu", &gemv_glu);
   m.impl("silu_mul", &silu_mul);
   m.impl("rope_tables", &rope_tables);
+  m.impl("pack_prompts", &pack_prompts);
+  m.impl("qk_rope_append", &qk_rope_append);
+  m.impl("prompt_attention", &prompt_attention);
+  m.impl("shared_decode", &shared_decode);
   m.impl("argmax_rows", &argmax_rows);
 }

@@ -29,26 +29,11 @@ from types import MethodType
 
 import torch
 import torch.nn.functional as F
-from torch.autograd import forward_ad
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
-from ._ops import ops
+from ._ops import ops, unwatched
 from .cache import DecodeKVCache
 from .retrieval import DenseDecoder, RetrievalConfig, SparseDecoder, check_step_health
-
-
-# looked up once: every wrapped call of an eager step asks them
-_compiling, _grad_on = torch.compiler.is_compiling, torch.is_grad_enabled
-_transforms, _modes = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
-_trace = torch._C._get_tracing_state
-
-
-def _unwatched() -> bool:
-    """Whether the calling ops only have to compute: no compiler, gradient, function
-    transform (vmap, jvp), forward-mode level, dispatch mode (fake tensors, op
-    counters) or trace looks at them, all of which a kernel call would pass by."""
-    return not (_compiling() or _grad_on() or forward_ad._current_level >= 0 or
-                _transforms() is not None or _modes() or _trace() is not None)
 
 
 def _plain_tensor(x: torch.Tensor) -> bool:
@@ -60,7 +45,7 @@ def _plain_tensor(x: torch.Tensor) -> bool:
 def _one_token(x: torch.Tensor) -> bool:
     """Whether x [B, 1, n] is a decode step's activation that the fused
     element-wise kernels serve; anything else keeps the model's own code."""
-    return (_unwatched() and x.dim() == 3 and x.shape[1] == 1 and x.numel() > 0 and x.is_cuda and
+    return (unwatched() and x.dim() == 3 and x.shape[1] == 1 and x.numel() > 0 and x.is_cuda and
             x.dtype in (torch.bfloat16, torch.float16) and _plain_tensor(x))
 
 

@@ -419,9 +419,13 @@ class DenseDecoder:
 
     @torch.no_grad()
     def step(self, q: torch.Tensor, keys: torch.Tensor, vals: torch.Tensor,
-             lengths=None) -> torch.Tensor:
+             lengths=None, shared_prefix: int = 0) -> torch.Tensor:
         """Attention over all cached tokens: keys.shape[2] of them, or
-        ``lengths[b]`` for sequence b (ragged batches)."""
+        ``lengths[b]`` for sequence b (ragged batches).
+
+        shared_prefix: the first so many tokens are the same in every sequence;
+        their rows of sequence 0 are read once for the whole batch, and the other
+        sequences' copies not at all."""
         if q.dim() == 4:
             q = q[:, :, 0, :]
         B, Hq, Hkv, D = self.B, self.Hq, self.Hkv, self.D
@@ -430,25 +434,51 @@ class DenseDecoder:
         if rows is not None and (len(set(rows)) > 1 or rows[0] != T):
             if max(rows) > T or min(rows) < 1:
                 raise RuntimeError("lengths must lie in [1, keys.shape[2]]")
+            if shared_prefix > min(rows):
+                raise RuntimeError(f"a shared prefix of {shared_prefix} tokens exceeds a "
+                                   f"sequence of {min(rows)}")
             if self._plans is None:
                 self._plans = PlanBuffer(B, q.device)
             if tuple(rows) != self._plan_key:
                 self._plans.upload([(t, t, 0, 0, 0, 0, 0, t) for t in rows])
                 self._plan_key = tuple(rows)
             pdev = self._plans.dev
+            if shared_prefix:
+                return self._shared(q, keys[:, :, :max(rows)], vals[:, :, :max(rows)],
+                                    shared_prefix, pdev)
             self._ops.attn_decode_ragged(q, keys, vals, None, Hkv, 0, pdev, 0, max(rows),
                                          1.0 / math.sqrt(D), self.out, self.ws)
             return self.out.unsqueeze(2)
+        if shared_prefix:
+            if shared_prefix > T:
+                raise RuntimeError(f"a shared prefix of {shared_prefix} tokens exceeds {T} keys")
+            return self._shared(q, keys, vals, shared_prefix, None)
         return self._dense_uniform(q, keys, vals)
+
+    def _shared(self, q, keys, vals, prefix: int, plans) -> torch.Tensor:
+        B, Hq, Hkv, D = self.B, self.Hq, self.Hkv, self.D
+        if prefix < 0 or q.shape != (B, Hq, D) or keys.shape[1] != Hkv:
+            raise RuntimeError("shared-prefix step: a prefix of at least 0 tokens and tensors of "
+                               "the decoder's geometry expected")
+        if q.data_ptr() % 16 or q.stride(2) != 1 or any(s % 8 for s in q.stride()[:2]):
+            q = q.contiguous()
+        need = N.size_query("lap_shared_attn_decode_workspace_size", B, Hq, Hkv, D, keys.shape[2],
+                            prefix)
+        # its size goes by the prefix and the keys; a captured graph keeps its own
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        self._ops.shared_decode(q, keys, vals, prefix, plans, 1.0 / math.sqrt(D), self.out, ws)
+        return self.out.unsqueeze(2)
 
     @torch.no_grad()
     def step_dev(self, q: torch.Tensor, keys: torch.Tensor, vals: torch.Tensor,
-                 plans: torch.Tensor) -> torch.Tensor:
+                 plans: torch.Tensor, shared_prefix: int = 0) -> torch.Tensor:
         """Dense decode with each sequence's length read from device plans
         (t_total, tail [0, t_total)); fixed launch arguments, as
-        SparseDecoder.step_dev."""
+        SparseDecoder.step_dev.  shared_prefix as in :meth:`step`."""
         if q.dim() == 4:
             q = q[:, :, 0, :]
+        if shared_prefix:
+            return self._shared(q, keys, vals, shared_prefix, plans)
         B, Hq, Hkv, D = self.B, self.Hq, self.Hkv, self.D
         T = keys.shape[2]
         self._ops.attn_decode_ragged(q, keys, vals, None, Hkv, 0, plans, 0, T,
