@@ -27,6 +27,8 @@ namespace lap {
 namespace {
 
 constexpr int kBN = 64;  // keys per tile
+// A lane's byte offset within a tile is 32 bits.
+constexpr int kMaxRowStride = 1 << 24;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
@@ -108,30 +110,213 @@ struct FlashTile {
   int split;
 };
 
-// The tile of 64 keys from kt, rows past the last key of the range repeat it.
+// Copies of key tiles straight into LDS, 16 bytes per lane: a wave writes 1 KB of
+// consecutive slots, and the lane's global address undoes the swizzle.  A lane's offset
+// within a tile does not change, so a copy costs a base in scalar registers and m0.
 template <int D, int NW>
-__device__ __forceinline__ void load_tile(char* s_dst, const uint16_t* base, int64_t st, int kt,
-                                          int last, int tid) {
-  constexpr int C = D / 8, PER = kBN * C / (64 * NW);
-  const int wave = tid >> 6, lane = tid & 63;
+struct TileCopy {
+  static constexpr int C = D / 8, PER = kBN * C / (64 * NW);
+  uint32_t off[PER];
+  uint32_t st;
+
+  __device__ __forceinline__ void init(int64_t stride, int tid) {
+    st = (uint32_t)stride;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int slot0 = (i * NW + wave) * 64, slot = slot0 + lane;
+    for (int i = 0; i < PER; ++i) off[i] = offset(i, tid, kBN - 1);
+  }
+  __device__ __forceinline__ uint32_t offset(int i, int tid, int last) const {
+    const int slot = (i * NW + (tid >> 6)) * 64 + (tid & 63);
     const int row = slot / C, chunk = (slot % C) ^ swz<D>(row);
-    const uint16_t* g = base + (int64_t)min(kt + row, last) * st + chunk * 8;
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                     (LAP_LDS void*)(s_dst + slot0 * 16), 16, 0, 0);
+    return (min(row, last) * st + chunk * 8) * 2;
+  }
+  // The tile whose first row is at base; rows past `last` repeat row `last`.
+  __device__ __forceinline__ void issue(const char* s_dst, const uint16_t* base, int last,
+                                        int tid) const {
+    const uint32_t lds = (uint32_t)(uintptr_t)(LAP_LDS const char*)s_dst + (tid >> 6) * 1024;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint32_t o = last < kBN - 1 ? offset(i, tid, last) : off[i];
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                   :
+                   : "v"(o), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds + i * NW * 1024))
+                   : "memory");
+    }
+  }
+};
+
+// The running state of a wave's 32 rows.
+template <int DT, int D>
+struct Rows {
+  i16x8 qf[D / 16];   // Q^T operand
+  f32x16 o[D / 32];   // o^T: rows d = 32 dc + (i & 3) + 8 (i >> 2) + 4 (lane / 32)
+  float m, l;         // maximum (log2, scaled; equal in the lane pair) and this lane's sum
+};
+
+// A row's maximum is raised only when a tile exceeds it by more than this, so weights
+// go up to 2^8 before the division by their sum: no rounding differs for it, and the
+// o^T registers are rescaled in few tiles.
+constexpr float kSlack = 8.f;
+
+// LDS addresses of a lane's operands, of which a step's differ by constants only.
+template <int D>
+struct LaneAddr {
+  uint32_t k[D / 16], v[D / 32][2];
+  __device__ __forceinline__ void init(const char* s_k, const char* s_v, int lane) {
+    constexpr int C = D / 8;
+    const uint32_t bk = (uint32_t)(uintptr_t)(LAP_LDS const char*)s_k;
+    const uint32_t bv = (uint32_t)(uintptr_t)(LAP_LDS const char*)s_v;
+    const int col = lane & 31, hl = lane >> 5, g16 = (lane >> 4) & 1, i16 = lane & 15;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      k[ks] = bk + (col * C + ((2 * ks + hl) ^ swz<D>(col))) * 16;
+#pragma unroll
+    for (int dc = 0; dc < D / 32; ++dc)
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const int r = 8 * jj + 4 * hl + (i16 >> 2);
+        const int chunk = 4 * dc + 2 * g16 + ((i16 & 3) >> 1);
+        v[dc][jj] = bv + (r * C + (chunk ^ swz<D>(r))) * 16 + (i16 & 1) * 8;
+      }
+  }
+};
+
+// One tile of keys in buffer BUF.  MASK: key kt + r counts for a row only below its
+// `end`, and w_min is the least of the wave's.
+template <int DT, int D, int BUF, bool MASK>
+__device__ __forceinline__ void step(Rows<DT, D>& w, const LaneAddr<D>& la, const char* s_v0,
+                                     float c, int kt, int end, int w_min, int hi, int lane) {
+  constexpr int KS = D / 16, DC = D / 32, C = D / 8, TILE = kBN * D * 2;
+  const int col = lane & 31, hl = lane >> 5;
+  f32x16 s[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const i16x8 kf = *(LAP_LDS const i16x8*)(uintptr_t)(la.k[ks] + BUF * TILE + h * 32 * D * 2);
+      s[h] = mfma32<DT>(kf, w.qf[ks], s[h]);
+    }
+  if constexpr (MASK) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (kt + h * 32 + (i & 3) + 8 * (i >> 2) + 4 * hl >= end) s[h][i] = -INFINITY;
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[h][i]);
+  {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
+                                                    __builtin_bit_cast(uint32_t, mx), false, false);
+    mx = fmaxf(__builtin_bit_cast(float, r[0]), __builtin_bit_cast(float, r[1])) * c;
+  }
+  if (__ballot(mx > w.m + kSlack)) {  // also where m is -inf and a score is not
+    const float m_new = mx > w.m + kSlack ? mx : w.m;
+    const float alpha = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - m_new);
+    w.m = m_new;
+    w.l *= alpha;
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w.o[dc][i] *= alpha;
+  }
+  const float base = MASK && w.m == -INFINITY ? 0.f : w.m;
+  float sum[2] = {0.f, 0.f};
+  uint32_t pk[16];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], c, -base));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i + 1], c, -base));
+      sum[0] += p0;
+      sum[1] += p1;
+      pk[8 * h + i / 2] = pack2<DT>(p0, p1);
+    }
+  w.l += sum[0] + sum[1];
+
+  if constexpr (MASK) {
+    // A value that is not finite in a row that some of these queries do not see must
+    // not reach them as 0 * inf: such a tile is summed key by key instead.
+    const char* s_v = s_v0 + BUF * TILE;
+    u16x2 top = {0, 0};
+    for (int i = lane; i < kBN * C; i += 64) {
+      if (kt + i / C < w_min) continue;
+      const uint4 x = *reinterpret_cast<const uint4*>(s_v + i * 16);
+      const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+    }
+    constexpr unsigned short kInf = DT == LAP_DTYPE_F16 ? 0x7c00 : 0x7f80;
+    if (__ballot(top[0] >= kInf || top[1] >= kInf)) {
+#pragma unroll 1
+      for (int r = 0; r < kBN && kt + r < hi; ++r) {
+        // the weight of key r: register 4 * (r / 8) + r % 4 of half r / 32, in the lane
+        // of the pair with hl = r / 4 % 2
+        const int want = (r >> 5) * 8 + ((r >> 3) & 3) * 2 + ((r & 3) >> 1);
+        uint32_t u = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) u = i == want ? pk[i] : u;
+        u = __shfl(u, col + 32 * ((r >> 2) & 1), 64);
+        const float p = ld16<DT>((uint16_t)(r & 1 ? u >> 16 : u));
+        const bool sees = kt + r < end;
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int d = 32 * dc + (i & 3) + 8 * (i >> 2) + 4 * hl;
+            const float x = ld16<DT>(*reinterpret_cast<const uint16_t*>(
+                s_v + (r * C + ((d >> 3) ^ swz<D>(r))) * 16 + (d & 7) * 2));
+            w.o[dc][i] = sees ? __builtin_fmaf(p, x, w.o[dc][i]) : w.o[dc][i];
+          }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    const uint4 pw = make_uint4(pk[4 * ks], pk[4 * ks + 1], pk[4 * ks + 2], pk[4 * ks + 3]);
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc) {
+      i16x4 vt[2];
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+        vt[jj] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (LAP_LDS i16x4*)(uintptr_t)(la.v[dc][jj] + BUF * TILE + ks * 16 * D * 2));
+      const i16x8 vf = {vt[0][0], vt[0][1], vt[0][2], vt[0][3],
+                        vt[1][0], vt[1][1], vt[1][2], vt[1][3]};
+      w.o[dc] = mfma32<DT>(vf, __builtin_bit_cast(i16x8, pw), w.o[dc]);
+    }
   }
 }
 
 template <int DT, int D, int NW, bool SHARED>
-__device__ __forceinline__ void flash(const FlashArgs& a, const FlashTile& t, char* s_k,
-                                      char* s_v) {
-  constexpr int KS = D / 16, DC = D / 32, C = D / 8;
+__device__ __forceinline__ void flash(const FlashArgs& a, const FlashTile& t,
+                                      const char* s_k0, const char* s_v0) {
+  constexpr int KS = D / 16, DC = D / 32, TILE = kBN * D * 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int col = lane & 31, hl = lane >> 5;
   const int row = wave * 32 + col, j = row / a.G, head = row - j * a.G;
   const bool live = j < t.n;
+
+  // Two buffers: the copies of a tile are in flight while the one before it is worked on.
+  TileCopy<D, NW> ck, cv;
+  ck.init(a.k_st, tid);
+  cv.init(a.v_st, tid);
+  const auto fetch = [&](int kt, int buf) {
+    const int last = t.hi - 1 - kt;
+    ck.issue(s_k0 + buf * TILE, t.k + (int64_t)kt * a.k_st, last, tid);
+    cv.issue(s_v0 + buf * TILE, t.v + (int64_t)kt * a.v_st, last, tid);
+  };
+  if (t.lo < t.hi) fetch(t.lo, 0);
+
   int lim, w_max, w_min;  // keys that this row, some row and every row of the wave sees
   if (SHARED && t.lens) {
     lim = live ? t.lens[j * kPlanInts + 1] : 0;
@@ -152,166 +337,78 @@ __device__ __forceinline__ void flash(const FlashArgs& a, const FlashTile& t, ch
   w_max = __builtin_amdgcn_readfirstlane(w_max);
   w_min = __builtin_amdgcn_readfirstlane(w_min);
 
-  i16x8 qf[KS];
+  Rows<DT, D> w;
+  LaneAddr<D> la;
+  la.init(s_k0, s_v0, lane);
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    qf[ks] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    w.qf[ks] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
     if (live)
-      qf[ks] = *reinterpret_cast<const i16x8*>(t.q + j * t.q_st + head * a.q_sh + ks * 16 + hl * 8);
+      w.qf[ks] =
+          *reinterpret_cast<const i16x8*>(t.q + j * t.q_st + head * a.q_sh + ks * 16 + hl * 8);
   }
-  f32x16 o[DC];
 #pragma unroll
   for (int dc = 0; dc < DC; ++dc)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[dc][i] = 0.f;
-  float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < 16; ++i) w.o[dc][i] = 0.f;
+  w.m = -INFINITY;
+  w.l = 0.f;
 
-  for (int kt = t.lo; kt < t.hi; kt += kBN) {
-    __syncthreads();
-    load_tile<D, NW>(s_k, t.k, a.k_st, kt, t.hi - 1, tid);
-    load_tile<D, NW>(s_v, t.v, a.v_st, kt, t.hi - 1, tid);
-    __syncthreads();
-    if (kt >= w_max) continue;
-    f32x16 s[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
-      const int r = h * 32 + col;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const i16x8 kf = *reinterpret_cast<const i16x8*>(
-            s_k + (r * C + ((2 * ks + hl) ^ swz<D>(r))) * 16);
-        s[h] = mfma32<DT>(kf, qf[ks], s[h]);
-      }
-    }
-    const int end = min(lim, t.hi);
-    const bool masked = kt + kBN > min(w_min, t.hi);
-    if (masked) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (kt + h * 32 + (i & 3) + 8 * (i >> 2) + 4 * hl >= end) s[h][i] = -INFINITY;
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[h][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float m_new = fmaxf(m, mx * a.c);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m - m_use);
-    float sum = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], a.c, -m_use));
-        s[h][i] = p;
-        sum += p;
-      }
-    l = __builtin_fmaf(l, alpha, sum);
-    m = m_new;
-#pragma unroll
-    for (int dc = 0; dc < DC; ++dc)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[dc][i] *= alpha;
-
-    uint32_t pk[16];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) pk[8 * h + i] = pack2<DT>(s[h][2 * i], s[h][2 * i + 1]);
-
-    // A value that is not finite in a row that some of these queries do not see must
-    // not reach them as 0 * inf: such a tile is summed key by key instead.
-    bool dirty = false;
-    if (masked) {
-      u16x2 top = {0, 0};
-      for (int i = lane; i < kBN * C; i += 64) {
-        const int r = i / C;
-        if (kt + r < w_min) continue;
-        const uint4 w = *reinterpret_cast<const uint4*>(s_v + i * 16);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
-      }
-      constexpr unsigned short kInf = DT == LAP_DTYPE_F16 ? 0x7c00 : 0x7f80;
-      dirty = __ballot(top[0] >= kInf || top[1] >= kInf) != 0;
-    }
-    if (!dirty) {
-      const int g16 = (lane >> 4) & 1, i16 = lane & 15;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const uint4 pw = make_uint4(pk[4 * ks], pk[4 * ks + 1], pk[4 * ks + 2], pk[4 * ks + 3]);
-#pragma unroll
-        for (int dc = 0; dc < DC; ++dc) {
-          i16x4 vt[2];
-#pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            const int r = 16 * ks + 8 * jj + 4 * hl + (i16 >> 2);
-            const int chunk = 4 * dc + 2 * g16 + ((i16 & 3) >> 1);
-            vt[jj] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (LAP_LDS i16x4*)(s_v + (r * C + (chunk ^ swz<D>(r))) * 16 + (i16 & 1) * 8));
-          }
-          const i16x8 vf = {vt[0][0], vt[0][1], vt[0][2], vt[0][3],
-                            vt[1][0], vt[1][1], vt[1][2], vt[1][3]};
-          o[dc] = mfma32<DT>(vf, __builtin_bit_cast(i16x8, pw), o[dc]);
-        }
-      }
-    } else {
-#pragma unroll 1
-      for (int r = 0; r < kBN && kt + r < t.hi; ++r) {
-        // the weight of key r: register 4 * (r / 8) + r % 4 of half r / 32, in the lane
-        // of the pair with hl = r / 4 % 2
-        const int want = (r >> 5) * 8 + ((r >> 3) & 3) * 2 + ((r & 3) >> 1);
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w = i == want ? pk[i] : w;
-        w = __shfl(w, col + 32 * ((r >> 2) & 1), 64);
-        const float p = ld16<DT>((uint16_t)(r & 1 ? w >> 16 : w));
-        const bool sees = kt + r < end;
-#pragma unroll
-        for (int dc = 0; dc < DC; ++dc)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int d = 32 * dc + (i & 3) + 8 * (i >> 2) + 4 * hl;
-            const float x = ld16<DT>(*reinterpret_cast<const uint16_t*>(
-                s_v + (r * C + ((d >> 3) ^ swz<D>(r))) * 16 + (d & 7) * 2));
-            o[dc][i] = sees ? __builtin_fmaf(p, x, o[dc][i]) : o[dc][i];
-          }
-      }
-    }
+  const int end = min(lim, t.hi);
+  const int whole = w_max > 0 ? min(w_min, t.hi) : t.lo;  // keys below it are all seen
+  // this wave's copies have arrived and its reads returned; then everybody's
+  const auto arrive = [&] {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // Tiles that every row of the wave sees, two at a time; then the rest.  Every wave
+  // passes one barrier per tile, wherever it is.
+  int kt = t.lo;
+  for (; kt + 2 * kBN <= whole; kt += 2 * kBN) {
+    arrive();
+    fetch(kt + kBN, 1);
+    step<DT, D, 0, false>(w, la, s_v0, a.c, kt, 0, 0, 0, lane);
+    arrive();
+    if (kt + 2 * kBN < t.hi) fetch(kt + 2 * kBN, 0);
+    step<DT, D, 1, false>(w, la, s_v0, a.c, kt, 0, 0, 0, lane);
+  }
+  for (; kt < t.hi; kt += 2 * kBN) {
+    arrive();
+    if (kt + kBN < t.hi) fetch(kt + kBN, 1);
+    if (kt < w_max) step<DT, D, 0, true>(w, la, s_v0, a.c, kt, end, w_min, t.hi, lane);
+    if (kt + kBN >= t.hi) break;
+    arrive();
+    if (kt + 2 * kBN < t.hi) fetch(kt + 2 * kBN, 0);
+    if (kt + kBN < w_max)
+      step<DT, D, 1, true>(w, la, s_v0, a.c, kt + kBN, end, w_min, t.hi, lane);
   }
 
-  l += __shfl_xor(l, 32, 64);
+  w.l += __shfl_xor(w.l, 32, 64);
   if (!live) return;
   if (a.nsplit == 1) {
     // weights that sum to zero (no key, or all scores -inf) give zeros
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = w.l == 0.f ? 0.f : 1.0f / w.l;
     uint16_t* op = t.out + j * t.o_st + head * a.o_sh;
 #pragma unroll
     for (int dc = 0; dc < DC; ++dc)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        uint2 w;
-        w.x = pack2<DT>(o[dc][4 * g] * inv, o[dc][4 * g + 1] * inv);
-        w.y = pack2<DT>(o[dc][4 * g + 2] * inv, o[dc][4 * g + 3] * inv);
-        *reinterpret_cast<uint2*>(op + 32 * dc + 8 * g + 4 * hl) = w;
+        uint2 x;
+        x.x = pack2<DT>(w.o[dc][4 * g] * inv, w.o[dc][4 * g + 1] * inv);
+        x.y = pack2<DT>(w.o[dc][4 * g + 2] * inv, w.o[dc][4 * g + 3] * inv);
+        *reinterpret_cast<uint2*>(op + 32 * dc + 8 * g + 4 * hl) = x;
       }
     return;
   }
   const int64_t at = (t.row0 + (int64_t)j * a.Hq + head) * a.nsplit + t.split;
-  if (hl == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+  if (hl == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(w.m, w.l);
 #pragma unroll
   for (int dc = 0; dc < DC; ++dc)
 #pragma unroll
     for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<float4*>(a.part_o + at * D + 32 * dc + 8 * g + 4 * hl) =
-          make_float4(o[dc][4 * g], o[dc][4 * g + 1], o[dc][4 * g + 2], o[dc][4 * g + 3]);
+      *reinterpret_cast<float4*>(a.part_o + at * D + 32 * dc + 8 * g + 4 * hl) = make_float4(
+          w.o[dc][4 * g], w.o[dc][4 * g + 1], w.o[dc][4 * g + 2], w.o[dc][4 * g + 3]);
 }
 
 // Tile ti of a prompt call: its sequence, first token (of the sequence in the uniform
@@ -338,7 +435,7 @@ __device__ __forceinline__ int64_t prompt_row(const FlashArgs& a, const PromptTi
 // to different XCDs, so an XCD's L2 holds the keys of few heads.
 template <int DT, int D, int NW>
 __global__ __launch_bounds__(64 * NW) void prompt_kernel(FlashArgs a) {
-  __shared__ __attribute__((aligned(256))) char s_k[kBN * D * 2], s_v[kBN * D * 2];
+  __shared__ __attribute__((aligned(256))) char s_k[2 * kBN * D * 2], s_v[2 * kBN * D * 2];
   const int hkv = blockIdx.x % a.Hkv;
   const int rest = blockIdx.x / a.Hkv;
   const int split = rest % a.nsplit;
@@ -370,7 +467,7 @@ __global__ __launch_bounds__(64 * NW) void prompt_kernel(FlashArgs a) {
 // splits of its own keys.
 template <int DT, int D, int NW>
 __global__ __launch_bounds__(64 * NW) void shared_kernel(FlashArgs a) {
-  __shared__ __attribute__((aligned(256))) char s_k[kBN * D * 2], s_v[kBN * D * 2];
+  __shared__ __attribute__((aligned(256))) char s_k[2 * kBN * D * 2], s_v[2 * kBN * D * 2];
   const int hkv = blockIdx.x % a.Hkv;
   const int it = blockIdx.x / a.Hkv, n_pre = a.psplit * a.pblocks;
   FlashTile t;
@@ -563,6 +660,8 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
   const uintptr_t ptrs = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(keys) |
                          reinterpret_cast<uintptr_t>(vals) | reinterpret_cast<uintptr_t>(out) |
                          reinterpret_cast<uintptr_t>(tiles);
+  LAP_CHECK(k_st >= 0 && v_st >= 0 && k_st <= kMaxRowStride && v_st <= kMaxRowStride,
+            "lap_prompt_attention: K/V row strides above %d", kMaxRowStride);
   LAP_CHECK((ptrs & 15) == 0 && ((q_sb | q_st | q_sh | k_sb | k_sh | k_st | v_sb | v_sh | v_st |
                                   o_sb | o_st | o_sh) & 7) == 0,
             "lap_prompt_attention: rows must be 16-byte aligned");
@@ -662,6 +761,8 @@ extern "C" int lap_shared_attn_decode(const void* q, int64_t q_sb, int64_t q_sh,
   LAP_CHECK(scale > 0.f && scale < INFINITY, "lap_shared_attn_decode: scale must be positive");
   const uintptr_t ptrs = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(keys) |
                          reinterpret_cast<uintptr_t>(vals) | reinterpret_cast<uintptr_t>(out);
+  LAP_CHECK(k_st >= 0 && v_st >= 0 && k_st <= kMaxRowStride && v_st <= kMaxRowStride,
+            "lap_shared_attn_decode: K/V row strides above %d", kMaxRowStride);
   LAP_CHECK((ptrs & 15) == 0 &&
                 ((q_sb | q_sh | k_sb | k_sh | k_st | v_sb | v_sh | v_st) & 7) == 0,
             "lap_shared_attn_decode: rows must be 16-byte aligned");
