@@ -548,8 +548,9 @@ int lap_argmax_rows(const void* x, int64_t x_row_stride, int rows, int V, int dt
  * lap_prompt_shape: the tile shape that the calls below take for `total`
  * packed tokens of B sequences, no sequence with more than max_keys cached and
  * new tokens: tokens per tile, an upper bound of the tiles, and the parts that
- * a tile's keys are split into (host arithmetic, no device call). */
-int lap_prompt_shape(int total, int B, int max_keys, int Hq, int Hkv, int D,
+ * a tile's keys are split into (host arithmetic, no device call).  tiles: their
+ * number where it is known (the lengths are), else 0. */
+int lap_prompt_shape(int total, int B, int tiles, int max_keys, int Hq, int Hkv, int D,
                      int* tokens_per_tile, int* n_tiles, int* nsplit);
 /* Tables from device lengths (B up to 4096; a length below zero counts as zero, tokens
  * past `total` are cut off):
@@ -598,7 +599,7 @@ int lap_qk_rope_append(const void* q, int64_t q_st, int64_t q_sh,
  *   tokens_per_tile, nsplit   of lap_prompt_shape; max_keys as given to it
  *   workspace   for nsplit > 1: lap_prompt_attention_workspace_size(tokens, ...), tokens =
  *           Tq (packed) or B * Tq.  Calls that share one must be ordered.
- * D 64, 128 or 256, fp16/bf16, Hq / Hkv up to 256, every row 16-byte aligned. */
+ * D 64, 128 or 256, fp16/bf16, Hq / Hkv up to 128, every row 16-byte aligned. */
 int lap_prompt_attention_workspace_size(int64_t tokens, int Hq, int D, int nsplit, size_t* bytes);
 int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                          const void* keys, const void* vals,
@@ -616,7 +617,7 @@ int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
  * read once, from sequence 0's rows, for all sequences; keys [prefix, len) are each
  * sequence's own.  len = min(plans[b].t_total, T), or T where plans is NULL; a sequence
  * shorter than the prefix sees len keys of it.  Other arguments and the output as
- * lap_dense_attn_decode; q and K/V rows 16-byte aligned, Hq / Hkv up to 256. */
+ * lap_dense_attn_decode; q and K/V rows 16-byte aligned, Hq / Hkv up to 128. */
 int lap_shared_attn_decode_workspace_size(int B, int Hq, int Hkv, int D, int T, int prefix,
                                           size_t* bytes);
 int lap_shared_attn_decode(const void* q, int64_t q_sb, int64_t q_sh,

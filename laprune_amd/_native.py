@@ -102,7 +102,7 @@ SIGNATURES = {
                         vp, i64, i64, i64, vp, vp],
     "lap_encode_keys_ranges": [vp, i32, i64, i64, i64, i32, i32, vp, i32, i32, i32, vp, i32, i32,
                                vp, sz, vp, i64, i64, i64, vp],
-    "lap_prompt_shape": [i32, i32, i32, i32, i32, i32, pint, pint, pint],
+    "lap_prompt_shape": [i32, i32, i32, i32, i32, i32, i32, pint, pint, pint],
     "lap_pack_prompts": [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp],
     "lap_qk_rope_append": [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp, i64, vp, f32, vp, f32,
                            i32, i64, i32, i32, i32, i32, vp, vp, vp, i64, i64, i64, vp, i64, i64,

@@ -78,7 +78,7 @@ def _prompt_kernel_fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bo
             k.dtype == q.dtype and v.dtype == q.dtype and q.device == k.device == v.device and
             q.shape[0] == k.shape[0] > 0 and k.shape[1] > 0 and q.shape[3] == k.shape[3] and
             q.shape[3] in (64, 128, 256) and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and
-            q.shape[1] // k.shape[1] <= 256 and 0 < q.shape[2] <= k.shape[2] and
+            q.shape[1] // k.shape[1] <= 128 and 0 < q.shape[2] <= k.shape[2] and
             all(type(t) in (torch.Tensor, torch.nn.Parameter) and _rows16(t) for t in (q, k, v)) and
             untraced() and not _needs_grad(q, k, v))
 
@@ -157,9 +157,11 @@ def do_sdpa_attn(query, key, value, cos=None, sin=None, out_proj=None, query_dow
     elif mask is None and num_queries > 1 and _prompt_kernel_fits(q, k, v):
         from .packed import prompt_shape
         B, Hq, Tq, D = q.shape
+        heads = Hq, k.shape[1], D
+        n = B * -(-Tq // prompt_shape(Tq, 1, k.shape[2], *heads)[0])
         output = q.new_empty((B, Tq, Hq, D))
         _prompt_launch(q.transpose(1, 2), k, v, None,
-                       prompt_shape(B * Tq, B, k.shape[2], Hq, k.shape[1], D), k.shape[2],
+                       prompt_shape(B * Tq, B, k.shape[2], *heads, n), k.shape[2],
                        1.0 / math.sqrt(D), output)
         output = output.transpose(1, 2)
     elif mask is not None:

@@ -26,7 +26,18 @@
 namespace lap {
 namespace {
 
-constexpr int kBN = 64;  // keys per tile
+// Rows of a workgroup: four waves of 32.  (Two waves, or eight, were slower or the same
+// at every size: one prompt of 16384 tokens, 32 query heads on 8, D = 128, 3146 and 2065
+// us against 2051; of 2048 68 and 67 against 57; of 512 18.3 and 22.8 against 17.8.)
+constexpr int NW = 4, kThreads = 64 * NW, kRows = 32 * NW;
+constexpr int kGran = 64;  // parts of the keys are multiples of this
+// Keys per tile.  At D = 256 a row's o^T takes 128 registers and its query 64: scores and
+// weights of 32 keys leave room for operands (64 keys spill: 5922 us against 3492 for a
+// prompt of 16384 tokens with 16 heads).
+template <int D>
+constexpr int bn() {
+  return D == 256 ? 32 : 64;
+}
 // A lane's byte offset within a tile is 32 bits.
 constexpr int kMaxRowStride = 1 << 24;
 
@@ -113,9 +124,9 @@ struct FlashTile {
 // Copies of key tiles straight into LDS, 16 bytes per lane: a wave writes 1 KB of
 // consecutive slots, and the lane's global address undoes the swizzle.  A lane's offset
 // within a tile does not change, so a copy costs a base in scalar registers and m0.
-template <int D, int NW>
+template <int D>
 struct TileCopy {
-  static constexpr int C = D / 8, PER = kBN * C / (64 * NW);
+  static constexpr int kBN = bn<D>(), C = D / 8, PER = kBN * C / (64 * NW);
   uint32_t off[PER];
   uint32_t st;
 
@@ -133,14 +144,19 @@ struct TileCopy {
   __device__ __forceinline__ void issue(const char* s_dst, const uint16_t* base, int last,
                                         int tid) const {
     const uint32_t lds = (uint32_t)(uintptr_t)(LAP_LDS const char*)s_dst + (tid >> 6) * 1024;
+    if (last >= kBN - 1) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const uint32_t o = last < kBN - 1 ? offset(i, tid, last) : off[i];
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                   :
-                   : "v"(o), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds + i * NW * 1024))
-                   : "memory");
+      for (int i = 0; i < PER; ++i) copy(lds + i * NW * 1024, base, off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) copy(lds + i * NW * 1024, base, offset(i, tid, last));
     }
+  }
+  static __device__ __forceinline__ void copy(uint32_t lds, const uint16_t* base, uint32_t o) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(o), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
+                 : "memory");
   }
 };
 
@@ -157,58 +173,81 @@ struct Rows {
 // o^T registers are rescaled in few tiles.
 constexpr float kSlack = 8.f;
 
-// LDS addresses of a lane's operands, of which a step's differ by constants only.
+// LDS addresses of a lane's operands in the first buffer.  The others are a constant
+// away, or, within a row, a constant XORed to the chunk's bits: rows of 128 bytes or
+// more, aligned to their size, and a swizzle that is an XOR.
 template <int D>
 struct LaneAddr {
-  uint32_t k[D / 16], v[D / 32][2];
+  uint32_t k, v[2];
   __device__ __forceinline__ void init(const char* s_k, const char* s_v, int lane) {
     constexpr int C = D / 8;
-    const uint32_t bk = (uint32_t)(uintptr_t)(LAP_LDS const char*)s_k;
-    const uint32_t bv = (uint32_t)(uintptr_t)(LAP_LDS const char*)s_v;
     const int col = lane & 31, hl = lane >> 5, g16 = (lane >> 4) & 1, i16 = lane & 15;
+    k = (uint32_t)(uintptr_t)(LAP_LDS const char*)s_k + (col * C + (hl ^ swz<D>(col))) * 16;
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-      k[ks] = bk + (col * C + ((2 * ks + hl) ^ swz<D>(col))) * 16;
-#pragma unroll
-    for (int dc = 0; dc < D / 32; ++dc)
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        const int r = 8 * jj + 4 * hl + (i16 >> 2);
-        const int chunk = 4 * dc + 2 * g16 + ((i16 & 3) >> 1);
-        v[dc][jj] = bv + (r * C + (chunk ^ swz<D>(r))) * 16 + (i16 & 1) * 8;
-      }
+    for (int jj = 0; jj < 2; ++jj) {
+      const int r = 8 * jj + 4 * hl + (i16 >> 2), chunk = 2 * g16 + ((i16 & 3) >> 1);
+      v[jj] = (uint32_t)(uintptr_t)(LAP_LDS const char*)s_v +
+              (r * C + (chunk ^ swz<D>(r))) * 16 + (i16 & 1) * 8;
+    }
   }
 };
 
-// One tile of keys in buffer BUF.  MASK: key kt + r counts for a row only below its
-// `end`, and w_min is the least of the wave's.
-template <int DT, int D, int BUF, bool MASK>
-__device__ __forceinline__ void step(Rows<DT, D>& w, const LaneAddr<D>& la, const char* s_v0,
-                                     float c, int kt, int end, int w_min, int hi, int lane) {
-  constexpr int KS = D / 16, DC = D / 32, C = D / 8, TILE = kBN * D * 2;
-  const int col = lane & 31, hl = lane >> 5;
-  f32x16 s[2];
+// An address as one register, so that what is added to it later is an instruction's
+// offset and not another register.
+__device__ __forceinline__ uint32_t pinned(uint32_t at) {
+  asm("" : "+v"(at));
+  return at;
+}
+
+// The three parts of a tile's work.  Buffers are named by their byte offset from the
+// first one.
+
+// Scores of the 64 keys of the K buffer at kb: their operands, and the products.
+template <int D>
+using KeyOps = i16x8[bn<D>() / 32][D / 16];
+template <int D>
+using Scores = f32x16[bn<D>() / 32];
+template <int D>
+using Weights = uint32_t[bn<D>() / 4];
+template <int D>
+__device__ __forceinline__ void load_keys(const LaneAddr<D>& la, uint32_t kb, KeyOps<D>& kf) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int ks = 0; ks < D / 16; ++ks) {
+    const uint32_t at = pinned((la.k + kb) ^ (ks << 5));
+#pragma unroll
+    for (int h = 0; h < bn<D>() / 32; ++h)
+      kf[h][ks] = *(LAP_LDS const i16x8*)(uintptr_t)(at + h * 32 * D * 2);
+  }
+}
+template <int DT, int D>
+__device__ __forceinline__ void scores(const Rows<DT, D>& w, const KeyOps<D>& kf, Scores<D>& s) {
+#pragma unroll
+  for (int h = 0; h < bn<D>() / 32; ++h)
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[h][i] = 0.f;
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
+  for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const i16x8 kf = *(LAP_LDS const i16x8*)(uintptr_t)(la.k[ks] + BUF * TILE + h * 32 * D * 2);
-      s[h] = mfma32<DT>(kf, w.qf[ks], s[h]);
-    }
+    for (int h = 0; h < bn<D>() / 32; ++h) s[h] = mfma32<DT>(kf[h][ks], w.qf[ks], s[h]);
+}
+
+// Scores -> weights pk (two to a register) and the rows' running state.  MASK: key
+// kt + r counts for a row only below its `end`.
+template <int DT, int D, bool MASK>
+__device__ __forceinline__ void weights(Rows<DT, D>& w, Scores<D>& s, Weights<D>& pk, float c,
+                                        int kt, int end, int lane) {
+  constexpr int DC = D / 32;
   if constexpr (MASK) {
+    const int left = end - kt - 4 * (lane >> 5);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < bn<D>() / 32; ++h)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (kt + h * 32 + (i & 3) + 8 * (i >> 2) + 4 * hl >= end) s[h][i] = -INFINITY;
+        s[h][i] = h * 32 + (i & 3) + 8 * (i >> 2) < left ? s[h][i] : -INFINITY;
   }
   float mx = s[0][0];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < bn<D>() / 32; ++h)
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[h][i]);
   {
@@ -222,15 +261,12 @@ __device__ __forceinline__ void step(Rows<DT, D>& w, const LaneAddr<D>& la, cons
     w.m = m_new;
     w.l *= alpha;
 #pragma unroll
-    for (int dc = 0; dc < DC; ++dc)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w.o[dc][i] *= alpha;
+    for (int dc = 0; dc < DC; ++dc) w.o[dc] *= alpha;
   }
-  const float base = MASK && w.m == -INFINITY ? 0.f : w.m;
+  const float base = w.m == -INFINITY ? 0.f : w.m;
   float sum[2] = {0.f, 0.f};
-  uint32_t pk[16];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < bn<D>() / 32; ++h)
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
       const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], c, -base));
@@ -240,56 +276,27 @@ __device__ __forceinline__ void step(Rows<DT, D>& w, const LaneAddr<D>& la, cons
       pk[8 * h + i / 2] = pack2<DT>(p0, p1);
     }
   w.l += sum[0] + sum[1];
+}
 
-  if constexpr (MASK) {
-    // A value that is not finite in a row that some of these queries do not see must
-    // not reach them as 0 * inf: such a tile is summed key by key instead.
-    const char* s_v = s_v0 + BUF * TILE;
-    u16x2 top = {0, 0};
-    for (int i = lane; i < kBN * C; i += 64) {
-      if (kt + i / C < w_min) continue;
-      const uint4 x = *reinterpret_cast<const uint4*>(s_v + i * 16);
-      const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+// o^T += V^T P^T of the 64 rows of the V buffer at vb.
+template <int DT, int D>
+__device__ __forceinline__ void values(Rows<DT, D>& w, const LaneAddr<D>& la, uint32_t vb,
+                                       const Weights<D>& pk) {
+  uint32_t at[D / 32][2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
-    }
-    constexpr unsigned short kInf = DT == LAP_DTYPE_F16 ? 0x7c00 : 0x7f80;
-    if (__ballot(top[0] >= kInf || top[1] >= kInf)) {
-#pragma unroll 1
-      for (int r = 0; r < kBN && kt + r < hi; ++r) {
-        // the weight of key r: register 4 * (r / 8) + r % 4 of half r / 32, in the lane
-        // of the pair with hl = r / 4 % 2
-        const int want = (r >> 5) * 8 + ((r >> 3) & 3) * 2 + ((r & 3) >> 1);
-        uint32_t u = 0;
+  for (int dc = 0; dc < D / 32; ++dc)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) u = i == want ? pk[i] : u;
-        u = __shfl(u, col + 32 * ((r >> 2) & 1), 64);
-        const float p = ld16<DT>((uint16_t)(r & 1 ? u >> 16 : u));
-        const bool sees = kt + r < end;
+    for (int jj = 0; jj < 2; ++jj) at[dc][jj] = pinned((la.v[jj] + vb) ^ (dc << 6));
 #pragma unroll
-        for (int dc = 0; dc < DC; ++dc)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int d = 32 * dc + (i & 3) + 8 * (i >> 2) + 4 * hl;
-            const float x = ld16<DT>(*reinterpret_cast<const uint16_t*>(
-                s_v + (r * C + ((d >> 3) ^ swz<D>(r))) * 16 + (d & 7) * 2));
-            w.o[dc][i] = sees ? __builtin_fmaf(p, x, w.o[dc][i]) : w.o[dc][i];
-          }
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
+  for (int ks = 0; ks < bn<D>() / 16; ++ks) {
     const uint4 pw = make_uint4(pk[4 * ks], pk[4 * ks + 1], pk[4 * ks + 2], pk[4 * ks + 3]);
 #pragma unroll
-    for (int dc = 0; dc < DC; ++dc) {
+    for (int dc = 0; dc < D / 32; ++dc) {
       i16x4 vt[2];
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj)
         vt[jj] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (LAP_LDS i16x4*)(uintptr_t)(la.v[dc][jj] + BUF * TILE + ks * 16 * D * 2));
+            (LAP_LDS i16x4*)(uintptr_t)(at[dc][jj] + ks * 16 * D * 2));
       const i16x8 vf = {vt[0][0], vt[0][1], vt[0][2], vt[0][3],
                         vt[1][0], vt[1][1], vt[1][2], vt[1][3]};
       w.o[dc] = mfma32<DT>(vf, __builtin_bit_cast(i16x8, pw), w.o[dc]);
@@ -297,23 +304,68 @@ __device__ __forceinline__ void step(Rows<DT, D>& w, const LaneAddr<D>& la, cons
   }
 }
 
-template <int DT, int D, int NW, bool SHARED>
+// The same of a tile that not every row of the wave sees in whole.  A value that is not
+// finite in a row that some of these queries do not see (from w_min on) must not reach
+// them as 0 * inf: such a tile is summed key by key instead.
+template <int DT, int D>
+__device__ __forceinline__ void values_masked(Rows<DT, D>& w, const LaneAddr<D>& la,
+                                              const char* s_v, uint32_t vb,
+                                              const Weights<D>& pk, int kt, int end, int w_min,
+                                              int hi, int lane) {
+  constexpr int DC = D / 32, C = D / 8, kBN = bn<D>();
+  const int col = lane & 31, hl = lane >> 5;
+  u16x2 top = {0, 0};
+  for (int i = lane; i < kBN * C; i += 64) {
+    if (kt + i / C < w_min) continue;
+    const uint4 x = *reinterpret_cast<const uint4*>(s_v + vb + i * 16);
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, u[e] & 0x7fff7fffu));
+  }
+  constexpr unsigned short kInf = DT == LAP_DTYPE_F16 ? 0x7c00 : 0x7f80;
+  if (!__ballot(top[0] >= kInf || top[1] >= kInf)) {
+    values<DT, D>(w, la, vb, pk);
+    return;
+  }
+#pragma unroll 1
+  for (int r = 0; r < kBN && kt + r < hi; ++r) {
+    // the weight of key r: register 4 * (r / 8) + r % 4 of half r / 32, in the lane of
+    // the pair with hl = r / 4 % 2
+    const int want = (r >> 5) * 8 + ((r >> 3) & 3) * 2 + ((r & 3) >> 1);
+    uint32_t u = 0;
+#pragma unroll
+    for (int i = 0; i < kBN / 4; ++i) u = i == want ? pk[i] : u;
+    u = __shfl(u, col + 32 * ((r >> 2) & 1), 64);
+    const float p = ld16<DT>((uint16_t)(r & 1 ? u >> 16 : u));
+    const bool sees = kt + r < end;
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int d = 32 * dc + (i & 3) + 8 * (i >> 2) + 4 * hl;
+        const float x = ld16<DT>(*reinterpret_cast<const uint16_t*>(
+            s_v + vb + (r * C + ((d >> 3) ^ swz<D>(r))) * 16 + (d & 7) * 2));
+        w.o[dc][i] = sees ? __builtin_fmaf(p, x, w.o[dc][i]) : w.o[dc][i];
+      }
+  }
+}
+
+template <int DT, int D, bool SHARED>
 __device__ __forceinline__ void flash(const FlashArgs& a, const FlashTile& t,
                                       const char* s_k0, const char* s_v0) {
-  constexpr int KS = D / 16, DC = D / 32, TILE = kBN * D * 2;
+  constexpr int kBN = bn<D>(), KS = D / 16, DC = D / 32, TILE = kBN * D * 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int col = lane & 31, hl = lane >> 5;
   const int row = wave * 32 + col, j = row / a.G, head = row - j * a.G;
   const bool live = j < t.n;
 
-  // Two buffers: the copies of a tile are in flight while the one before it is worked on.
-  TileCopy<D, NW> ck, cv;
+  TileCopy<D> ck, cv;
   ck.init(a.k_st, tid);
   cv.init(a.v_st, tid);
-  const auto fetch = [&](int kt, int buf) {
-    const int last = t.hi - 1 - kt;
-    ck.issue(s_k0 + buf * TILE, t.k + (int64_t)kt * a.k_st, last, tid);
-    cv.issue(s_v0 + buf * TILE, t.v + (int64_t)kt * a.v_st, last, tid);
+  const auto fetch = [&](int kt, uint32_t buf) {
+    ck.issue(s_k0 + buf, t.k + (int64_t)kt * a.k_st, t.hi - 1 - kt, tid);
+    cv.issue(s_v0 + buf, t.v + (int64_t)kt * a.v_st, t.hi - 1 - kt, tid);
   };
   if (t.lo < t.hi) fetch(t.lo, 0);
 
@@ -356,32 +408,39 @@ __device__ __forceinline__ void flash(const FlashArgs& a, const FlashTile& t,
 
   const int end = min(lim, t.hi);
   const int whole = w_max > 0 ? min(w_min, t.hi) : t.lo;  // keys below it are all seen
-  // this wave's copies have arrived and its reads returned; then everybody's
-  const auto arrive = [&] {
+  // Two buffers: the copies of a tile are in flight while the one before it is worked on.
+  Scores<D> s;
+  Weights<D> pk;
+  KeyOps<D> kf;
+  uint32_t buf = 0;
+  const auto begin = [&](int kt) {
+    // this wave's copies have come and its reads are done; then everybody's
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    if (kt + kBN < t.hi) fetch(kt + kBN, buf ^ TILE);
   };
-  // Tiles that every row of the wave sees, two at a time; then the rest.  Every wave
-  // passes one barrier per tile, wherever it is.
   int kt = t.lo;
-  for (; kt + 2 * kBN <= whole; kt += 2 * kBN) {
-    arrive();
-    fetch(kt + kBN, 1);
-    step<DT, D, 0, false>(w, la, s_v0, a.c, kt, 0, 0, 0, lane);
-    arrive();
-    if (kt + 2 * kBN < t.hi) fetch(kt + 2 * kBN, 0);
-    step<DT, D, 1, false>(w, la, s_v0, a.c, kt, 0, 0, 0, lane);
+  for (; kt + kBN <= whole; kt += kBN, buf ^= TILE) {
+    begin(kt);
+    load_keys<D>(la, buf, kf);
+    // products before the other workgroup's weights: 2066 us against 2108 (a prompt of
+    // 16384 tokens, 32 heads on 8, D = 128)
+    __builtin_amdgcn_s_setprio(1);
+    scores<DT, D>(w, kf, s);
+    __builtin_amdgcn_s_setprio(0);
+    weights<DT, D, false>(w, s, pk, a.c, kt, 0, lane);
+    __builtin_amdgcn_s_setprio(1);
+    values<DT, D>(w, la, buf, pk);
+    __builtin_amdgcn_s_setprio(0);
   }
-  for (; kt < t.hi; kt += 2 * kBN) {
-    arrive();
-    if (kt + kBN < t.hi) fetch(kt + kBN, 1);
-    if (kt < w_max) step<DT, D, 0, true>(w, la, s_v0, a.c, kt, end, w_min, t.hi, lane);
-    if (kt + kBN >= t.hi) break;
-    arrive();
-    if (kt + 2 * kBN < t.hi) fetch(kt + 2 * kBN, 0);
-    if (kt + kBN < w_max)
-      step<DT, D, 1, true>(w, la, s_v0, a.c, kt + kBN, end, w_min, t.hi, lane);
+  for (; kt < t.hi; kt += kBN, buf ^= TILE) {  // every wave passes a barrier per tile
+    begin(kt);
+    if (kt >= w_max) continue;
+    load_keys<D>(la, buf, kf);
+    scores<DT, D>(w, kf, s);
+    weights<DT, D, true>(w, s, pk, a.c, kt, end, lane);
+    values_masked<DT, D>(w, la, s_v0, buf, pk, kt, end, w_min, t.hi, lane);
   }
 
   w.l += __shfl_xor(w.l, 32, 64);
@@ -433,9 +492,11 @@ __device__ __forceinline__ int64_t prompt_row(const FlashArgs& a, const PromptTi
 
 // Workgroup -> (tile, split, KV head), the KV head fastest: consecutive workgroups go
 // to different XCDs, so an XCD's L2 holds the keys of few heads.
-template <int DT, int D, int NW>
-__global__ __launch_bounds__(64 * NW) void prompt_kernel(FlashArgs a) {
-  __shared__ __attribute__((aligned(256))) char s_k[2 * kBN * D * 2], s_v[2 * kBN * D * 2];
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+void prompt_kernel(FlashArgs a) {
+  __shared__ __attribute__((aligned(256))) char s_k[2 * bn<D>() * D * 2],
+      s_v[2 * bn<D>() * D * 2];
   const int hkv = blockIdx.x % a.Hkv;
   const int rest = blockIdx.x / a.Hkv;
   const int split = rest % a.nsplit;
@@ -458,16 +519,18 @@ __global__ __launch_bounds__(64 * NW) void prompt_kernel(FlashArgs a) {
   t.split = split;
   t.lo = (int)min((int64_t)split * a.per_split, (int64_t)keys);
   t.hi = split == a.nsplit - 1 ? keys : min(keys, t.lo + a.per_split);
-  flash<DT, D, NW, false>(a, t, s_k, s_v);
+  flash<DT, D, false>(a, t, s_k, s_v);
 }
 
 // One query token per sequence over keys of which the first `prefix` are the same in
 // every sequence.  Items: for the prefix, blocks of as many sequences as fill the
 // workgroup's rows, by splits of the keys of sequence 0; behind it, each sequence by
 // splits of its own keys.
-template <int DT, int D, int NW>
-__global__ __launch_bounds__(64 * NW) void shared_kernel(FlashArgs a) {
-  __shared__ __attribute__((aligned(256))) char s_k[2 * kBN * D * 2], s_v[2 * kBN * D * 2];
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+void shared_kernel(FlashArgs a) {
+  __shared__ __attribute__((aligned(256))) char s_k[2 * bn<D>() * D * 2],
+      s_v[2 * bn<D>() * D * 2];
   const int hkv = blockIdx.x % a.Hkv;
   const int it = blockIdx.x / a.Hkv, n_pre = a.psplit * a.pblocks;
   FlashTile t;
@@ -498,47 +561,69 @@ __global__ __launch_bounds__(64 * NW) void shared_kernel(FlashArgs a) {
   t.o_st = (int64_t)a.Hq * D;
   t.k = a.k + (int64_t)kb * a.k_sb + (int64_t)hkv * a.k_sh;
   t.v = a.v + (int64_t)kb * a.v_sb + (int64_t)hkv * a.v_sh;
-  flash<DT, D, NW, true>(a, t, s_k, s_v);
+  flash<DT, D, true>(a, t, s_k, s_v);
 }
 
-// out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) of one row: four waves take the
-// splits in turn, a lane D / 64 of the row's values.
+// out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) of one row: a wave, its lanes D / 64
+// of the row's values each, kMergeAhead splits' values in flight.
+constexpr int kMergeRows = 4, kMergeAhead = 8;
+template <int D>
+struct Vals;
+template <> struct Vals<64> { typedef float type; };
+template <> struct Vals<128> { typedef float2 type; };
+template <> struct Vals<256> { typedef float4 type; };
+
 template <int DT, int D>
 __device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, uint16_t* out) {
   constexpr int V = D / 64;
-  __shared__ float s_o[4][D], s_l[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float* ml = a.part_ml + row * a.nsplit * 2;
-  float M = -INFINITY;
-  for (int s = lane; s < a.nsplit; s += 64) M = fmaxf(M, ml[2 * s]);
+  typedef typename Vals<D>::type vals;
+  const int lane = threadIdx.x & 63;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.nsplit;
+  const vals* po = reinterpret_cast<const vals*>(a.part_o + row * a.nsplit * D) + lane;
+  // 64 splits at a time: lane s holds split s's weight
+  float M = -INFINITY, l = 0.f, o[V] = {};
+  for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
+    const int n = min(64, a.nsplit - s0);
+    const float2 x = lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+    float top = x.x;
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
-  const float base = M == -INFINITY ? 0.f : M;
-  float o[V] = {}, l = 0.f;
-  const float* po = a.part_o + row * a.nsplit * D + lane * V;
-  for (int s = wave; s < a.nsplit; s += 4) {
-    const float ls = ml[2 * s + 1];
-    if (ls == 0.f) continue;  // nothing of this row in the split
-    const float w = __builtin_amdgcn_exp2f(ml[2 * s] - base);
-    l = __builtin_fmaf(ls, w, l);
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    top = fmaxf(top, M);
+    const float base = top == -INFINITY ? 0.f : top;
+    // a split without keys of this row: weight 0, and its values are 0
+    const float w = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - base);
+    const float before = __builtin_amdgcn_exp2f(M - base);
+    float sum = x.y * w;
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(po[(int64_t)s * D + e], w, o[e]);
+    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    l = l * before + sum;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] *= before;
+    M = top;
+    for (int s = 0; s < n; s += kMergeAhead) {
+      vals v[kMergeAhead];
+#pragma unroll
+      for (int i = 0; i < kMergeAhead; ++i) v[i] = po[(int64_t)(s0 + min(s + i, n - 1)) * 64];
+#pragma unroll
+      for (int i = 0; i < kMergeAhead; ++i) {
+        const float ws = s + i < n ? __shfl(w, s + i, 64) : 0.f;
+        const float* f = reinterpret_cast<const float*>(&v[i]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = ws == 0.f ? o[e] : __builtin_fmaf(f[e], ws, o[e]);
+      }
+    }
   }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-  for (int e = 0; e < V; ++e) s_o[wave][lane * V + e] = o[e];
-  if (lane == 0) s_l[wave] = l;
-  __syncthreads();
-  if (tid >= D) return;
-  const float all = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-  const float x = s_o[0][tid] + s_o[1][tid] + s_o[2][tid] + s_o[3][tid];
-  out[tid] = st16<DT>(all == 0.f ? 0.f : x / all);
+  for (int e = 0; e < V; ++e) out[lane * V + e] = st16<DT>(o[e] * inv);
 }
 
-// One workgroup per (tile, token, head); only rows of a tile are written.
+// One wave per (tile, token, head); only rows of a tile are written.
 template <int DT, int D>
-__global__ __launch_bounds__(256) void prompt_merge_kernel(FlashArgs a) {
-  const int h = blockIdx.x % a.Hq, rest = blockIdx.x / a.Hq;
-  const int j = rest % a.bt;
+__global__ __launch_bounds__(64 * kMergeRows) void prompt_merge_kernel(FlashArgs a, int rows) {
+  const int r = blockIdx.x * kMergeRows + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int h = r % a.Hq, rest = r / a.Hq, j = rest % a.bt;
   PromptTile p;
   if (!prompt_tile(a, rest / a.bt, p) || j >= p.n) return;
   uint16_t* out = a.out + (a.tiles ? 0 : p.b) * a.o_sb + (int64_t)(p.q0 + j) * a.o_st + h * a.o_sh;
@@ -546,47 +631,39 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(FlashArgs a) {
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(256) void shared_merge_kernel(FlashArgs a) {
-  merge_row<DT, D>(a, blockIdx.x, a.out + (int64_t)blockIdx.x * D);
+__global__ __launch_bounds__(64 * kMergeRows) void shared_merge_kernel(FlashArgs a, int rows) {
+  const int r = blockIdx.x * kMergeRows + (threadIdx.x >> 6);
+  if (r < rows) merge_row<DT, D>(a, r, a.out + (int64_t)r * D);
 }
 
-#define LAP_BY_NW(KERNEL)                                                              \
-  do {                                                                                \
-    if (nw == 1) hipLaunchKernelGGL((KERNEL<DT, D, 1>), g, dim3(64), 0, st, a);       \
-    else if (nw == 2) hipLaunchKernelGGL((KERNEL<DT, D, 2>), g, dim3(128), 0, st, a); \
-    else if (nw == 4) hipLaunchKernelGGL((KERNEL<DT, D, 4>), g, dim3(256), 0, st, a); \
-    else hipLaunchKernelGGL((KERNEL<DT, D, 8>), g, dim3(512), 0, st, a);              \
-  } while (0)
-
-// The kernel and, with more than one split, the merge.
+// The kernel and, with more than one split, the merge of `rows` rows.
 template <bool SHARED, int DT, int D>
-int launch_flash(const FlashArgs& a, int nw, int64_t grid, int64_t merge_grid, hipStream_t st) {
-  const dim3 g((unsigned)grid), mg((unsigned)merge_grid);
-  if constexpr (SHARED) LAP_BY_NW(shared_kernel);
-  else LAP_BY_NW(prompt_kernel);
+int launch_flash(const FlashArgs& a, int64_t grid, int64_t rows, hipStream_t st) {
+  const dim3 g((unsigned)grid), mg((unsigned)((rows + kMergeRows - 1) / kMergeRows));
+  if constexpr (SHARED) hipLaunchKernelGGL((shared_kernel<DT, D>), g, dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((prompt_kernel<DT, D>), g, dim3(kThreads), 0, st, a);
   LAP_LAUNCH_CHECK("attention of many rows");
   if (a.nsplit > 1) {
-    if constexpr (SHARED) hipLaunchKernelGGL((shared_merge_kernel<DT, D>), mg, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((prompt_merge_kernel<DT, D>), mg, dim3(256), 0, st, a);
+    const dim3 threads(64 * kMergeRows);
+    if constexpr (SHARED)
+      hipLaunchKernelGGL((shared_merge_kernel<DT, D>), mg, threads, 0, st, a, (int)rows);
+    else hipLaunchKernelGGL((prompt_merge_kernel<DT, D>), mg, threads, 0, st, a, (int)rows);
     LAP_LAUNCH_CHECK("merge of splits");
   }
   return LAP_OK;
 }
-#undef LAP_BY_NW
 
 template <bool SHARED>
-int launch_by_type(const FlashArgs& a, int dtype, int D, int nw, int64_t grid, int64_t merge_grid,
+int launch_by_type(const FlashArgs& a, int dtype, int D, int64_t grid, int64_t rows,
                    hipStream_t st) {
-#define LAP_BY_D(DT)                                                             \
-  return D == 64    ? launch_flash<SHARED, DT, 64>(a, nw, grid, merge_grid, st)  \
-         : D == 128 ? launch_flash<SHARED, DT, 128>(a, nw, grid, merge_grid, st) \
-                    : launch_flash<SHARED, DT, 256>(a, nw, grid, merge_grid, st)
+#define LAP_BY_D(DT)                                                  \
+  return D == 64    ? launch_flash<SHARED, DT, 64>(a, grid, rows, st)  \
+         : D == 128 ? launch_flash<SHARED, DT, 128>(a, grid, rows, st) \
+                    : launch_flash<SHARED, DT, 256>(a, grid, rows, st)
   if (dtype == LAP_DTYPE_F16) LAP_BY_D(LAP_DTYPE_F16);
   LAP_BY_D(LAP_DTYPE_BF16);
 #undef LAP_BY_D
 }
-
-int waves_of(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }
 
 size_t part_bytes(int64_t rows, int nsplit, int D) {
   return nsplit > 1 ? (size_t)rows * nsplit * (D + 2) * sizeof(float) : 0;
@@ -595,8 +672,8 @@ size_t part_bytes(int64_t rows, int nsplit, int D) {
 int check_heads(const char* fn, int Hq, int Hkv, int D) {
   LAP_CHECK(Hq > 0 && Hkv > 0 && D > 0, "%s: bad sizes", fn);
   LAP_CHECK(Hq % Hkv == 0, "invalid GQA head counts: Hq=%d, Hkv=%d", Hq, Hkv);
-  LAP_CHECK_CODE(Hq / Hkv <= 256, LAP_ERR_UNSUPPORTED, "%s: group size %d unsupported (1 to 256)",
-                 fn, Hq / Hkv);
+  LAP_CHECK_CODE(Hq / Hkv <= kRows, LAP_ERR_UNSUPPORTED, "%s: group size %d unsupported (1 to %d)",
+                 fn, Hq / Hkv, kRows);
   LAP_CHECK_CODE(D == 64 || D == 128 || D == 256, LAP_ERR_UNSUPPORTED,
                  "%s: head dim %d unsupported (64/128/256)", fn, D);
   return LAP_OK;
@@ -607,26 +684,25 @@ int check_heads(const char* fn, int Hq, int Hkv, int D) {
 
 using namespace lap;
 
-extern "C" int lap_prompt_shape(int total, int B, int max_keys, int Hq, int Hkv, int D,
-                                int* tokens_per_tile, int* n_tiles, int* nsplit) {
+extern "C" int lap_prompt_shape(int total, int B, int tiles, int max_keys, int Hq, int Hkv,
+                                int D, int* tokens_per_tile, int* n_tiles, int* nsplit) {
   clear_error();
   LAP_CHECK(tokens_per_tile && n_tiles && nsplit, "lap_prompt_shape: null output");
   LAP_CHECK(total >= 0 && B > 0 && max_keys >= 0, "lap_prompt_shape: bad sizes");
   int s = check_heads("lap_prompt_shape", Hq, Hkv, D);
   if (s != LAP_OK) return s;
-  constexpr int kCUs = 256;
-  const int G = Hq / Hkv;
-  int nw = 8;
-  auto tiles_of = [&](int w) { return (int64_t)total / (32 * w / G) + std::min(B, total); };
-  while (nw > 1 && 32 * (nw / 2) >= G && tiles_of(nw) * Hkv < 2 * kCUs) nw /= 2;
-  const int64_t items = tiles_of(nw) * Hkv;
+  const int bt = kRows / (Hq / Hkv), bound = total / bt + std::min(B, total);
+  // 512 workgroups run at a time (two to a CU).  Fewer than 256 of them share out the
+  // keys, at least 512 each: a part below costs more in the merge than it gives, and a
+  // 513th workgroup starts when the others are done (300 tokens behind 36057, 68
+  // workgroups: 6 parts 198 us, 8 parts 265; 512 tokens, 136 workgroups: 1 part 17.8, 2
+  // parts of 256 39.6).
+  const int64_t items = (int64_t)(tiles > 0 ? std::min(tiles, bound) : bound) * Hkv;
   int ns = 1;
-  if (items < 2 * kCUs && items > 0) {
-    ns = (int)std::min<int64_t>(2 * kCUs / items, ((int64_t)max_keys + 255) / 256);
-    ns = std::max(1, std::min(ns, 256));
-  }
-  *tokens_per_tile = 32 * nw / G;
-  *n_tiles = (int)tiles_of(nw);
+  if (items > 0 && items < 256)
+    ns = (int)std::max<int64_t>(1, std::min<int64_t>({512 / items, max_keys / 512, 32}));
+  *tokens_per_tile = bt;
+  *n_tiles = bound;
   *nsplit = ns;
   return LAP_OK;
 }
@@ -666,7 +742,7 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
                                   o_sb | o_st | o_sh) & 7) == 0,
             "lap_prompt_attention: rows must be 16-byte aligned");
   const int G = Hq / Hkv;
-  LAP_CHECK(tokens_per_tile > 0 && (int64_t)tokens_per_tile * G <= 256 && nsplit > 0 &&
+  LAP_CHECK(tokens_per_tile > 0 && (int64_t)tokens_per_tile * G <= kRows && nsplit > 0 &&
                 n_tiles >= 0 && max_keys >= 0,
             "lap_prompt_attention: bad tile shape");
   if (!tiles) n_tiles = B * ((Tq + tokens_per_tile - 1) / tokens_per_tile);
@@ -683,7 +759,7 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
   a.bt = tokens_per_tile;
   a.tps = (Tq + tokens_per_tile - 1) / tokens_per_tile;
   a.nsplit = nsplit;
-  a.per_split = (std::max(1, (std::min(max_keys, Tk) + nsplit - 1) / nsplit) + kBN - 1) / kBN * kBN;
+  a.per_split = (std::max(1, (std::min(max_keys, Tk) + nsplit - 1) / nsplit) + kGran - 1) / kGran * kGran;
   a.c = scale * kLog2e;
   a.out = static_cast<uint16_t*>(out);
   a.o_sb = o_sb; a.o_st = o_st; a.o_sh = o_sh;
@@ -698,7 +774,7 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + rows * nsplit * D;
   }
-  return launch_by_type<false>(a, dtype, D, waves_of(tokens_per_tile * G), grid,
+  return launch_by_type<false>(a, dtype, D, grid,
                                (int64_t)n_tiles * tokens_per_tile * Hq, as_stream(stream));
 }
 
@@ -707,18 +783,16 @@ namespace {
 
 // Rows per block, keys per split and splits of a decode step over a shared prefix.
 struct SharedShape {
-  int nw, bt, pblocks, per, psplit, nsplit;
+  int bt, pblocks, per, psplit, nsplit;
 };
 SharedShape shared_shape(int B, int Hkv, int G, int T, int prefix) {
   constexpr int kItems = 1024;
   SharedShape s;
-  s.nw = waves_of((int)std::min<int64_t>((int64_t)B * G, 256));
-  while (32 * s.nw < G) s.nw *= 2;
-  s.bt = 32 * s.nw / G;
+  s.bt = kRows / G;
   s.pblocks = (B + s.bt - 1) / s.bt;
   const int64_t keys = ((int64_t)s.pblocks * prefix + (int64_t)B * (T - prefix)) * Hkv;
   int64_t per = std::max<int64_t>({128, (keys + kItems - 1) / kItems, (T + 511) / 512});
-  s.per = (int)((per + kBN - 1) / kBN * kBN);
+  s.per = (int)((per + kGran - 1) / kGran * kGran);
   s.psplit = (prefix + s.per - 1) / s.per;
   s.nsplit = s.psplit + (T - prefix + s.per - 1) / s.per;
   return s;
@@ -796,5 +870,5 @@ extern "C" int lap_shared_attn_decode(const void* q, int64_t q_sb, int64_t q_sh,
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + rows * sh.nsplit * D;
   }
-  return launch_by_type<true>(a, dtype, D, sh.nw, grid, rows, as_stream(stream));
+  return launch_by_type<true>(a, dtype, D, grid, rows, as_stream(stream));
 }

@@ -20,10 +20,11 @@ from ._ops import ops
 
 @functools.lru_cache(1024)
 def prompt_shape(total: int, batch: int, max_keys: int, num_q_heads: int, num_kv_heads: int,
-                 head_dim: int) -> tuple[int, int, int]:
-    """(tokens per tile, bound of the tiles, parts of a tile's keys) of a pass."""
+                 head_dim: int, tiles: int = 0) -> tuple[int, int, int]:
+    """(tokens per tile, bound of the tiles, parts of a tile's keys) of a pass; tiles:
+    their number, when the lengths are known."""
     out = [C.c_int(0) for _ in range(3)]
-    N.call("lap_prompt_shape", total, batch, max_keys, num_q_heads, num_kv_heads, head_dim,
+    N.call("lap_prompt_shape", total, batch, tiles, max_keys, num_q_heads, num_kv_heads, head_dim,
            *map(C.byref, out))
     return tuple(v.value for v in out)
 
@@ -108,6 +109,9 @@ def pack_prompts(lens, cached=None, total: int | None = None, max_keys: int | No
             raise ValueError("pack_prompts: num_q_heads, num_kv_heads and head_dim go together")
         heads = num_q_heads, num_kv_heads, head_dim
         shape = prompt_shape(total, B, max_keys, *heads)
+        if host[0] is not None:
+            n = sum(-(-t // shape[0]) for t in host[0])
+            shape = prompt_shape(total, B, max_keys, *heads, n)
         tiles = torch.empty((shape[1], 4), dtype=torch.int32, device=dev)
     starts = torch.empty(B + 1, dtype=torch.int32, device=dev)
     seq = torch.empty(total, dtype=torch.int32, device=dev)

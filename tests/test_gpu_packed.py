@@ -209,7 +209,7 @@ PROMPTS = [  # heads, new, cached
     ((3, 3, 256), [70, 1], [0, 0]),
     ((8, 1, 256), [33, 130], [129, 0]),
     ((40, 1, 64), [9, 30], [5, 0]),       # more heads than a wave has rows
-    ((256, 1, 64), [3], [10]),            # one token fills a workgroup's rows
+    ((128, 1, 256), [3], [10]),           # one token fills a workgroup's rows
     ((16, 8, 64), [700, 300, 411], [0, 0, 64]),
 ]
 
@@ -226,16 +226,16 @@ def test_prompt_attention(dev, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("waves", [1, 2, 4, 8])
+@pytest.mark.parametrize("rows", [3, 32, 100, 128])
 @pytest.mark.parametrize("nsplit", [1, 2, 5])
 @pytest.mark.parametrize("D", [64, 128, 256])
-def test_every_tile_shape_and_split(dev, dtype, waves, nsplit, D):
+def test_every_tile_shape_and_split(dev, dtype, rows, nsplit, D):
     """Each tile height, with the keys whole and in parts (some of them empty)."""
     from laprune_amd import packed
     from laprune_amd.attention import prompt_attention
     Hq, Hkv, lens, cached = 6, 2, [150, 1, 61], [0, 300, 7]
-    q, k, v = _attn_case(dev, dtype, Hq, Hkv, D, lens, cached, seed=waves)
-    bt = 32 * waves // 3
+    q, k, v = _attn_case(dev, dtype, Hq, Hkv, D, lens, cached, seed=rows)
+    bt = rows // 3
     shape = (bt, sum(lens) // bt + len(lens), nsplit)
     plan = packed.pack_prompts(lens, cached, device=dev, num_q_heads=Hq, num_kv_heads=Hkv, head_dim=D)
     plan.shape, plan.tiles = shape, torch.empty((shape[1], 4), dtype=torch.int32, device=dev)
@@ -468,7 +468,7 @@ def test_refusals_on_the_gpu(dev):
     bad(x, k, v, plan, match="aligned")
     with pytest.raises(RuntimeError, match="tile"):
         from laprune_amd._ops import ops
-        ops().prompt_attention(q, k, v, plan.tiles, 129, 1, 10, 0.1, torch.empty_like(q), None)
+        ops().prompt_attention(q, k, v, plan.tiles, 65, 1, 10, 0.1, torch.empty_like(q), None)
     c = _cache(dev, torch.bfloat16, 1, 2, 64, 16)
     rq, rk, rv, cos, sin, _ = _rope_inputs(dev, torch.bfloat16, 10, 4, 2, 64)
     with pytest.raises(RuntimeError, match="tokens expected"):

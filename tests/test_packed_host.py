@@ -16,18 +16,18 @@ def _err(lib):
     return lib.lap_last_error().decode()
 
 
-@pytest.mark.parametrize("heads", [(1, 1, 64), (32, 8, 128), (28, 4, 128), (256, 1, 64), (40, 1, 256),
+@pytest.mark.parametrize("heads", [(1, 1, 64), (32, 8, 128), (28, 4, 128), (128, 1, 64), (40, 1, 256),
                                    (8, 8, 256), (33, 1, 64)])
 @pytest.mark.parametrize("total,B,keys", [(0, 1, 0), (1, 1, 1), (7, 3, 70000), (777, 7, 400),
                                           (16384, 1, 16384), (131072, 256, 131072), (1, 1, 1 << 29)])
 def test_prompt_shape(heads, total, B, keys):
-    """A tile's rows fit a workgroup (32 to 256), the bound holds every split of the
+    """A tile's rows fit a workgroup (128), the bound holds every split of the
     tokens over the sequences, and no part of the keys is without keys at the longest."""
     from laprune_amd.packed import prompt_shape
     Hq, Hkv, D = heads
     bt, n, ns = prompt_shape(total, B, keys, Hq, Hkv, D)
     G = Hq // Hkv
-    assert bt >= 1 and bt * G <= 256 and ns >= 1
+    assert bt >= 1 and bt * G <= 128 and ns >= 1
     assert n >= total // bt + min(B, total)
     assert ns == 1 or keys > 64 * (ns - 1)
 
@@ -86,10 +86,10 @@ def test_invalid_arguments_of_the_c_abi(lib):
 
     for kw, code, msg in [(dict(q=null), 1, "null"), (dict(dtype=N.F32), 1, "fp16/bf16"),
                           (dict(Hq=7), 1, "GQA"), (dict(D=96), 2, "head dim"),
-                          (dict(Hq=257, Hkv=1), 2, "group size"), (dict(Tq=10), 1, "exceed"),
+                          (dict(Hq=129, Hkv=1), 2, "group size"), (dict(Tq=10), 1, "exceed"),
                           (dict(scale=-1.0), 1, "scale"), (dict(scale=float("inf")), 1, "scale"),
                           (dict(q=odd), 1, "aligned"), (dict(st=1025), 1, "aligned"),
-                          (dict(bt=65), 1, "tile"), (dict(bt=0), 1, "tile"), (dict(ns=0), 1, "tile"),
+                          (dict(bt=33), 1, "tile"), (dict(bt=0), 1, "tile"), (dict(ns=0), 1, "tile"),
                           (dict(ns=2), 4, "workspace"), (dict(ns=2, ws=al, wsb=100), 4, "workspace"),
                           (dict(Tk=1 << 30), 1, "sizes")]:
         assert prompt(**kw) == code and msg in _err(lib), kw
@@ -104,9 +104,9 @@ def test_invalid_arguments_of_the_c_abi(lib):
                           (dict(Hq=9), 1, "GQA"), (dict(D=80), 2, "head dim"), (dict(scale=0.0), 1, "scale"),
                           (dict(q=odd), 1, "aligned"), (dict(kst=132), 1, "aligned"), (dict(), 4, "workspace")]:
         assert shared(**kw) == code and msg in _err(lib), kw
-    assert lib.lap_prompt_shape(-1, 1, 1, 8, 2, 64, C.byref(i), C.byref(i), C.byref(i)) == 1
-    assert lib.lap_prompt_shape(1, 1, 1, 8, 3, 64, C.byref(i), C.byref(i), C.byref(i)) == 1
-    assert lib.lap_prompt_shape(1, 1, 1, 8, 2, 96, C.byref(i), C.byref(i), C.byref(i)) == 2
+    assert lib.lap_prompt_shape(-1, 1, 0, 1, 8, 2, 64, C.byref(i), C.byref(i), C.byref(i)) == 1
+    assert lib.lap_prompt_shape(1, 1, 0, 1, 8, 3, 64, C.byref(i), C.byref(i), C.byref(i)) == 1
+    assert lib.lap_prompt_shape(1, 1, 0, 1, 8, 2, 96, C.byref(i), C.byref(i), C.byref(i)) == 2
 
 
 def test_workspace_sizes(lib):
