@@ -23,7 +23,6 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import _native as N
 from ._ops import ops, untraced
 
 
@@ -83,16 +82,6 @@ def _prompt_kernel_fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bo
             untraced() and not _needs_grad(q, k, v))
 
 
-def _prompt_launch(q, k, v, tiles, shape, max_keys: int, scale: float, out) -> None:
-    Hq, D = q.shape[-2:]
-    tokens = q.numel() // (Hq * D)
-    ws = None
-    if shape[2] > 1:
-        need = N.size_query("lap_prompt_attention_workspace_size", tokens, Hq, D, shape[2])
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    ops().prompt_attention(q, k, v, tiles, shape[0], shape[2], max_keys, scale, out, ws)
-
-
 def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, plan,
                      scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of packed prompts over their caches.
@@ -127,8 +116,9 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise RuntimeError("prompt_attention: out must be like query")
     if plan.total:
-        _prompt_launch(q, k, v, plan.tiles, plan.shape, plan.max_keys,
-                       1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale), out)
+        bt, _, nsplit = plan.shape
+        ops().prompt_attention(q, k, v, plan.tiles, bt, nsplit, plan.max_keys,
+                               1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale), out)
     return out
 
 
@@ -159,10 +149,10 @@ def do_sdpa_attn(query, key, value, cos=None, sin=None, out_proj=None, query_dow
         B, Hq, Tq, D = q.shape
         heads = Hq, k.shape[1], D
         n = B * -(-Tq // prompt_shape(Tq, 1, k.shape[2], *heads)[0])
+        bt, _, nsplit = prompt_shape(B * Tq, B, k.shape[2], *heads, n)
         output = q.new_empty((B, Tq, Hq, D))
-        _prompt_launch(q.transpose(1, 2), k, v, None,
-                       prompt_shape(B * Tq, B, k.shape[2], *heads, n), k.shape[2],
-                       1.0 / math.sqrt(D), output)
+        ops().prompt_attention(q.transpose(1, 2), k, v, None, bt, nsplit, k.shape[2],
+                               1.0 / math.sqrt(D), output)
         output = output.transpose(1, 2)
     elif mask is not None:
         output = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, is_causal=False,

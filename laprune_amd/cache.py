@@ -258,6 +258,11 @@ class DecodeKVCache:
         rotation; norm and rotation are then computed in fp32 and rounded once."""
         D, B = self.D, self.B
         Hq = q.shape[-1] // D
+        if q_norm is not None or k_norm is not None:
+            if pos.numel() != B or q_out.shape != (B, Hq, D):
+                raise RuntimeError("rope_append: one position and q_out row per sequence")
+            self._qk_rope(q, k, v, cos, sin, None, pos, q_norm, k_norm, q_out)
+            return q_out.unsqueeze(2)
         if any(t.stride(-1) != 1 for t in (q, k, v, cos, sin)):
             raise RuntimeError("rope_append: rows must be contiguous")
         if any(t.dtype != self.dtype for t in (q, k, v, cos, sin)):
@@ -272,17 +277,12 @@ class DecodeKVCache:
             raise RuntimeError("rope_append: pos must be int64 with one position per sequence")
         if q_out.shape != (B, Hq, D) or not q_out.is_contiguous() or q_out.dtype != self.dtype:
             raise RuntimeError("rope_append: q_out must be a contiguous [B, Hq, D] tensor")
-        if q_norm is not None or k_norm is not None:
-            self._qk_rope(q, k, v, cos, sin, None, pos.reshape(B), q_norm, k_norm, q_out)
-            return q_out.unsqueeze(2)
         ops().rope_append(q, k, v, cos, sin, pos, self.k, self.v, self.capacity, q_out)
         return q_out.unsqueeze(2)
 
     def _qk_rope(self, q, k, v, cos, sin, seq, pos, q_norm, k_norm, q_out) -> None:
-        D, n = self.D, pos.numel()
         (qw, qe), (kw, ke) = q_norm or (None, 0.0), k_norm or (None, 0.0)
-        ops().qk_rope_append(*(x.reshape(n, -1, D) for x in (q, k, v)), cos.reshape(n, D),
-                             sin.reshape(n, D), qw, qe, kw, ke, seq, pos, self.k, self.v, q_out)
+        ops().qk_rope_append(q, k, v, cos, sin, qw, qe, kw, ke, seq, pos, self.k, self.v, q_out)
 
     @torch.no_grad()
     def rope_append_packed(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -301,18 +301,8 @@ class DecodeKVCache:
         D, n = self.D, plan.total
         if plan.B != self.B:
             raise RuntimeError(f"rope_append_packed: a plan of {plan.B} sequences, not {self.B}")
-        if any(t.dtype != self.dtype for t in (q, k, v, cos, sin)):
-            raise RuntimeError("rope_append_packed: q, k, v, cos and sin must be in the cache dtype")
-        if (any(t.numel() != n * t.shape[-1] for t in (q, k, v, cos, sin)) or q.shape[-1] % D
-                or k.shape[-1] != self.Hkv * D or v.shape[-1] != self.Hkv * D
-                or cos.shape[-1] != D or sin.shape[-1] != D):
-            raise RuntimeError("rope_append_packed: q [n, Hq*D], k/v [n, Hkv*D], cos/sin [n, D] "
-                               f"of n = {n} tokens expected")
-        Hq = q.shape[-1] // D
         if q_out is None:
-            q_out = q.new_empty((n, Hq, D))
-        elif q_out.shape != (n, Hq, D) or not q_out.is_contiguous() or q_out.dtype != self.dtype:
-            raise RuntimeError("rope_append_packed: q_out must be a contiguous [n, Hq, D] tensor")
+            q_out = q.new_empty((n, q.shape[-1] // D, D))
         if n:
             self._qk_rope(q, k, v, cos, sin, plan.seq, plan.pos, q_norm, k_norm, q_out)
         return q_out

@@ -564,90 +564,121 @@ void shared_kernel(FlashArgs a) {
   flash<DT, D, true>(a, t, s_k, s_v);
 }
 
-// out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) of one row: a wave, its lanes D / 64
-// of the row's values each, kMergeAhead splits' values in flight.
-constexpr int kMergeRows = 4, kMergeAhead = 8;
+// out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) of one row by WPR waves: a wave takes
+// every WPR-th batch of kMergeAhead splits, its lanes D / 64 of the row's values each, and
+// the first wave adds the waves up.  Four waves where there are more than kMergeFew splits
+// (their batches come one after the other), one where there are few (a decode step of 8
+// sequences behind 30000 tokens, 8 heads on 1: 33.2 us with one wave, 20.0 with four; a
+// prompt of 300 tokens behind 36057, 7 splits: 192.7 and 200.0).
+constexpr int kMergeAhead = 8, kMergeFew = 16, kMergeThreads = 256;
 template <int D>
 struct Vals;
 template <> struct Vals<64> { typedef float type; };
 template <> struct Vals<128> { typedef float2 type; };
 template <> struct Vals<256> { typedef float4 type; };
 
-template <int DT, int D>
-__device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, uint16_t* out) {
+template <int DT, int D, int WPR>
+__device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, bool live,
+                                          uint16_t* out) {
   constexpr int V = D / 64;
   typedef typename Vals<D>::type vals;
-  const int lane = threadIdx.x & 63;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.nsplit;
-  const vals* po = reinterpret_cast<const vals*>(a.part_o + row * a.nsplit * D) + lane;
-  // 64 splits at a time: lane s holds split s's weight
+  const int lane = threadIdx.x & 63, part = (threadIdx.x >> 6) % WPR;
   float M = -INFINITY, l = 0.f, o[V] = {};
-  for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
-    const int n = min(64, a.nsplit - s0);
-    const float2 x = lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
-    float top = x.x;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    top = fmaxf(top, M);
-    const float base = top == -INFINITY ? 0.f : top;
-    // a split without keys of this row: weight 0, and its values are 0
-    const float w = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - base);
-    const float before = __builtin_amdgcn_exp2f(M - base);
-    float sum = x.y * w;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    l = l * before + sum;
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] *= before;
-    M = top;
-    for (int s = 0; s < n; s += kMergeAhead) {
+  if (live) {
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.nsplit;
+    const vals* po = reinterpret_cast<const vals*>(a.part_o + row * a.nsplit * D) + lane;
+    // 64 splits at a time: lane s holds split s's weight
+    for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
+      const int n = min(64, a.nsplit - s0);
+      const float2 x = lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
       vals v[kMergeAhead];
+      const auto request = [&](int s) {
 #pragma unroll
-      for (int i = 0; i < kMergeAhead; ++i) v[i] = po[(int64_t)(s0 + min(s + i, n - 1)) * 64];
+        for (int i = 0; i < kMergeAhead; ++i) v[i] = po[(int64_t)(s0 + min(s + i, n - 1)) * 64];
+      };
+      int s = part * kMergeAhead;
+      if (s < n) request(s);
+      float top = x.x;
 #pragma unroll
-      for (int i = 0; i < kMergeAhead; ++i) {
-        const float ws = s + i < n ? __shfl(w, s + i, 64) : 0.f;
-        const float* f = reinterpret_cast<const float*>(&v[i]);
+      for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+      top = fmaxf(top, M);
+      const float base = top == -INFINITY ? 0.f : top;
+      // a split without keys of this row: weight 0, and its values are 0
+      const float w = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - base);
+      const float before = __builtin_amdgcn_exp2f(M - base);
+      float sum = x.y * w;
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = ws == 0.f ? o[e] : __builtin_fmaf(f[e], ws, o[e]);
+      for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+      l = l * before + sum;
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] *= before;
+      M = top;
+      while (s < n) {
+#pragma unroll
+        for (int i = 0; i < kMergeAhead; ++i) {
+          const float ws = s + i < n ? __shfl(w, s + i, 64) : 0.f;
+          const float* f = reinterpret_cast<const float*>(&v[i]);
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[e] = ws == 0.f ? o[e] : __builtin_fmaf(f[e], ws, o[e]);
+        }
+        s += WPR * kMergeAhead;
+        if (s < n) request(s);
       }
     }
   }
+  if constexpr (WPR > 1) {  // every wave has the same maxima and sum
+    __shared__ float s_o[WPR - 1][D];
+    if (part > 0)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s_o[part - 1][lane * V + e] = o[e];
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll
+    for (int p = 0; p < WPR - 1; ++p)
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] += s_o[p][lane * V + e];
+  }
+  if (!live) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
   for (int e = 0; e < V; ++e) out[lane * V + e] = st16<DT>(o[e] * inv);
 }
 
-// One wave per (tile, token, head); only rows of a tile are written.
-template <int DT, int D>
-__global__ __launch_bounds__(64 * kMergeRows) void prompt_merge_kernel(FlashArgs a, int rows) {
-  const int r = blockIdx.x * kMergeRows + (threadIdx.x >> 6);
-  if (r >= rows) return;
+// A row per (tile, token, head); only rows of a tile are written.
+template <int DT, int D, int WPR>
+__global__ __launch_bounds__(kMergeThreads) void prompt_merge_kernel(FlashArgs a, int rows) {
+  const int r = blockIdx.x * (4 / WPR) + (threadIdx.x >> 6) / WPR;
   const int h = r % a.Hq, rest = r / a.Hq, j = rest % a.bt;
-  PromptTile p;
-  if (!prompt_tile(a, rest / a.bt, p) || j >= p.n) return;
+  PromptTile p{};
+  const bool live = r < rows && prompt_tile(a, rest / a.bt, p) && j < p.n;
   uint16_t* out = a.out + (a.tiles ? 0 : p.b) * a.o_sb + (int64_t)(p.q0 + j) * a.o_st + h * a.o_sh;
-  merge_row<DT, D>(a, (prompt_row(a, p) + j) * a.Hq + h, out);
+  merge_row<DT, D, WPR>(a, (prompt_row(a, p) + j) * a.Hq + h, live, out);
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(64 * kMergeRows) void shared_merge_kernel(FlashArgs a, int rows) {
-  const int r = blockIdx.x * kMergeRows + (threadIdx.x >> 6);
-  if (r < rows) merge_row<DT, D>(a, r, a.out + (int64_t)r * D);
+template <int DT, int D, int WPR>
+__global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(FlashArgs a, int rows) {
+  const int r = blockIdx.x * (4 / WPR) + (threadIdx.x >> 6) / WPR;
+  merge_row<DT, D, WPR>(a, r, r < rows, a.out + (int64_t)r * D);
+}
+
+template <bool SHARED, int DT, int D, int WPR>
+void launch_merge(const FlashArgs& a, int64_t rows, hipStream_t st) {
+  const dim3 g((unsigned)((rows * WPR + 3) / 4)), threads(kMergeThreads);
+  if constexpr (SHARED)
+    hipLaunchKernelGGL((shared_merge_kernel<DT, D, WPR>), g, threads, 0, st, a, (int)rows);
+  else hipLaunchKernelGGL((prompt_merge_kernel<DT, D, WPR>), g, threads, 0, st, a, (int)rows);
 }
 
 // The kernel and, with more than one split, the merge of `rows` rows.
 template <bool SHARED, int DT, int D>
 int launch_flash(const FlashArgs& a, int64_t grid, int64_t rows, hipStream_t st) {
-  const dim3 g((unsigned)grid), mg((unsigned)((rows + kMergeRows - 1) / kMergeRows));
+  const dim3 g((unsigned)grid);
   if constexpr (SHARED) hipLaunchKernelGGL((shared_kernel<DT, D>), g, dim3(kThreads), 0, st, a);
   else hipLaunchKernelGGL((prompt_kernel<DT, D>), g, dim3(kThreads), 0, st, a);
   LAP_LAUNCH_CHECK("attention of many rows");
   if (a.nsplit > 1) {
-    const dim3 threads(64 * kMergeRows);
-    if constexpr (SHARED)
-      hipLaunchKernelGGL((shared_merge_kernel<DT, D>), mg, threads, 0, st, a, (int)rows);
-    else hipLaunchKernelGGL((prompt_merge_kernel<DT, D>), mg, threads, 0, st, a, (int)rows);
+    if (a.nsplit > kMergeFew) launch_merge<SHARED, DT, D, 4>(a, rows, st);
+    else launch_merge<SHARED, DT, D, 1>(a, rows, st);
     LAP_LAUNCH_CHECK("merge of splits");
   }
   return LAP_OK;
@@ -781,20 +812,30 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
 namespace lap {
 namespace {
 
-// Rows per block, keys per split and splits of a decode step over a shared prefix.
+// Rows per block, keys per split and splits of a decode step over a shared prefix.  512
+// workgroups run at a time; a workgroup's start, its first copies and its part of the
+// merge cost about as much as six tiles of 64 keys (64 sequences
+// behind 2000 tokens with up to 2000 of their own: 54.1 us, 70.6 if counted as three).
 struct SharedShape {
   int bt, pblocks, per, psplit, nsplit;
 };
 SharedShape shared_shape(int B, int Hkv, int G, int T, int prefix) {
-  constexpr int kItems = 1024;
-  SharedShape s;
+  SharedShape s{};
   s.bt = kRows / G;
   s.pblocks = (B + s.bt - 1) / s.bt;
-  const int64_t keys = ((int64_t)s.pblocks * prefix + (int64_t)B * (T - prefix)) * Hkv;
-  int64_t per = std::max<int64_t>({128, (keys + kItems - 1) / kItems, (T + 511) / 512});
-  s.per = (int)((per + kGran - 1) / kGran * kGran);
-  s.psplit = (prefix + s.per - 1) / s.per;
-  s.nsplit = s.psplit + (T - prefix + s.per - 1) / s.per;
+  int64_t least = INT64_MAX;
+  for (int64_t tiles = 2; tiles <= 4 || tiles * kGran < 2 * (int64_t)T; tiles += tiles / 4 + 1) {
+    const int64_t per = tiles * kGran, p = (prefix + per - 1) / per,
+                  n = p + (T - prefix + per - 1) / per;
+    const int64_t items = (p * s.pblocks + (n - p) * B) * Hkv;
+    const int64_t cost = (items + 511) / 512 * (tiles + 6);
+    if (cost < least && n <= 1024) {
+      least = cost;
+      s.per = (int)std::min<int64_t>(per, 1 << 30);
+      s.psplit = (int)p;
+      s.nsplit = (int)n;
+    }
+  }
   return s;
 }
 

@@ -12,12 +12,14 @@
 // built with hipcc against the torch headers, linked to the HIP library.
 #include <torch/library.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
 #include <cmath>
 #include <optional>
+#include <tuple>
 
 #include "../../include/laprune_hip.h"
 
@@ -335,37 +337,52 @@ void argmax_rows(const at::Tensor& x, const at::Tensor& out,
 
 // Packed prompts and decode over a shared prefix (csrc/pack.hip, csrc/cache.hip,
 // csrc/prompt.hip).  The calls run on the tensors' device, current or not.
-void pack_prompts(const at::Tensor& new_lens, const std::optional<at::Tensor>& cached,
-                  int64_t total, int64_t tokens_per_tile, const at::Tensor& starts,
-                  const at::Tensor& seq, const at::Tensor& pos,
-                  const std::optional<at::Tensor>& tiles) {
-  same_gpu("laprune::pack_prompts", {&new_lens, opt(cached), &starts, &seq, &pos, opt(tiles)});
+
+// -> starts [B + 1], seq [total], pos [total] and, with n_tiles >= 0, tiles [n_tiles, 4].
+std::tuple<at::Tensor, at::Tensor, at::Tensor, std::optional<at::Tensor>> pack_prompts(
+    const at::Tensor& new_lens, const std::optional<at::Tensor>& cached, int64_t total,
+    int64_t tokens_per_tile, int64_t n_tiles) {
+  same_gpu("laprune::pack_prompts", {&new_lens, opt(cached)});
   const int64_t B = new_lens.numel();
   TORCH_CHECK(new_lens.scalar_type() == at::kInt && new_lens.dim() == 1 &&
                   new_lens.is_contiguous() &&
                   (!cached || (cached->scalar_type() == at::kInt && cached->is_contiguous() &&
                                cached->dim() == 1 && cached->numel() == B)),
               "laprune::pack_prompts: int32 lengths [B]");
-  TORCH_CHECK(starts.scalar_type() == at::kInt && starts.is_contiguous() &&
-                  starts.numel() == B + 1 && seq.scalar_type() == at::kInt &&
-                  seq.is_contiguous() && seq.numel() == total && pos.scalar_type() == at::kLong &&
-                  pos.is_contiguous() && pos.numel() == total && B <= INT32_MAX &&
-                  total <= INT32_MAX &&
-                  (!tiles || (tiles->scalar_type() == at::kInt && tiles->is_contiguous() &&
-                              tiles->dim() == 2 && tiles->size(1) == 4)),
-              "laprune::pack_prompts: starts int32 [B + 1], seq int32 and pos int64 [total], "
-              "tiles int32 [n, 4]");
-  const c10::DeviceGuard guard(starts.device());
+  TORCH_CHECK(B <= INT32_MAX && total >= 0 && total <= INT32_MAX && n_tiles <= INT32_MAX,
+              "laprune::pack_prompts: bad sizes");
+  const c10::DeviceGuard guard(new_lens.device());
+  const auto ints = new_lens.options();
+  at::Tensor starts = at::empty({B + 1}, ints), seq = at::empty({total}, ints),
+             pos = at::empty({total}, ints.dtype(at::kLong));
+  std::optional<at::Tensor> tiles;
+  if (n_tiles >= 0) tiles = at::empty({n_tiles, 4}, ints);
   check(lap_pack_prompts(static_cast<const int32_t*>(ptr(new_lens)),
                          static_cast<const int32_t*>(ptr(cached)), (int)B, (int)total,
-                         (int)tokens_per_tile, tiles ? (int)tiles->size(0) : 0,
+                         (int)tokens_per_tile, tiles ? (int)n_tiles : 0,
                          static_cast<int32_t*>(ptr(starts)), static_cast<int32_t*>(ptr(seq)),
                          static_cast<int64_t*>(ptr(pos)), static_cast<int32_t*>(ptr(tiles)),
                          stream_of(starts)),
         "lap_pack_prompts");
+  return {starts, seq, pos, tiles};
 }
 
-// q [n, Hq, D], k / v [n, Hkv, D], cos / sin [n, D] or [1, D], caches [B, Hkv, T, D].
+// The stride between tokens of x [..., W] with n tokens in its leading dimensions.
+int64_t token_stride(const char* op, const at::Tensor& x, int64_t n) {
+  TORCH_CHECK(x.dim() >= 2 && x.numel() == n * x.size(-1) && x.stride(-1) == 1, op, ": rows of ",
+              n, " tokens expected, each contiguous");
+  int64_t st = 0, next = 0;  // next: the stride an outer dimension must have
+  for (int64_t d = x.dim() - 2; d >= 0; --d) {
+    if (x.size(d) == 1) continue;
+    TORCH_CHECK(!next || x.stride(d) == next, op, ": tokens must lie at one stride");
+    if (!next) st = x.stride(d);
+    next = x.stride(d) * x.size(d);
+  }
+  return st;
+}
+
+// q [..., Hq * D], k / v [..., Hkv * D], cos / sin [..., D] of n tokens each, caches
+// [B, Hkv, T, D], q_out [n, Hq, D].
 void qk_rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                     const at::Tensor& cos, const at::Tensor& sin,
                     const std::optional<at::Tensor>& q_weight, double q_eps,
@@ -373,38 +390,38 @@ void qk_rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
                     const std::optional<at::Tensor>& seq, const at::Tensor& pos,
                     const at::Tensor& cache_k, const at::Tensor& cache_v,
                     const at::Tensor& q_out) {
-  same_gpu("laprune::qk_rope_append", {&q, &k, &v, &cos, &sin, opt(q_weight), opt(k_weight),
-                                       opt(seq), &pos, &cache_k, &cache_v, &q_out});
-  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && cos.dim() == 2 && sin.dim() == 2 &&
-                  cache_k.dim() == 4 && cache_v.dim() == 4,
-              "laprune::qk_rope_append: q [n, Hq, D], k / v [n, Hkv, D], cos / sin [n, D], "
-              "caches [B, Hkv, T, D]");
-  const int64_t n = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
-  const auto dt = q.scalar_type();
-  for (const at::Tensor* t : {&q, &k, &v, &cos, &sin, &cache_k, &cache_v, &q_out})
-    TORCH_CHECK(t->scalar_type() == dt && t->size(-1) == D && t->stride(-1) == 1,
-                "laprune::qk_rope_append: one dtype, contiguous rows of head dim ", D);
-  TORCH_CHECK(k.size(0) == n && v.size(0) == n && v.size(1) == Hkv && cos.size(0) == n &&
-                  sin.size(0) == n && (n < 2 || sin.stride(0) == cos.stride(0)) &&
-                  q_out.is_contiguous() && q_out.numel() == n * Hq * D,
-              "laprune::qk_rope_append: one row of q, k, v, cos, sin and q_out per token");
-  TORCH_CHECK(cache_k.size(1) == Hkv && cache_v.sizes() == cache_k.sizes() &&
-                  cache_k.size(2) <= INT32_MAX,
-              "laprune::qk_rope_append: caches [B, Hkv, T, D] of one shape");
-  TORCH_CHECK(pos.scalar_type() == at::kLong && pos.is_contiguous() && pos.numel() == n &&
+  const char* op = "laprune::qk_rope_append";
+  same_gpu(op, {&q, &k, &v, &cos, &sin, opt(q_weight), opt(k_weight), opt(seq), &pos, &cache_k,
+                &cache_v, &q_out});
+  TORCH_CHECK(cache_k.dim() == 4 && cache_v.sizes() == cache_k.sizes() &&
+                  cache_k.stride(3) == 1 && cache_v.stride(3) == 1 && cache_k.size(2) <= INT32_MAX,
+              op, ": caches [B, Hkv, T, D] of one shape");
+  const int64_t n = pos.numel(), Hkv = cache_k.size(1), D = cache_k.size(3);
+  const auto dt = cache_k.scalar_type();
+  for (const at::Tensor* t : {&q, &k, &v, &cos, &sin, &cache_v, &q_out})
+    TORCH_CHECK(t->scalar_type() == dt, op, ": tensors must be in the cache dtype");
+  TORCH_CHECK(D > 0 && q.size(-1) % D == 0 && k.size(-1) == Hkv * D && v.size(-1) == Hkv * D &&
+                  cos.size(-1) == D && sin.size(-1) == D,
+              op, ": q [n, Hq * D], k / v [n, Hkv * D] and cos / sin [n, D] expected");
+  const int64_t Hq = q.size(-1) / D;
+  const int64_t q_st = token_stride(op, q, n), k_st = token_stride(op, k, n),
+                v_st = token_stride(op, v, n), cs_st = token_stride(op, cos, n);
+  TORCH_CHECK(token_stride(op, sin, n) == cs_st, op, ": cos and sin of equal strides");
+  TORCH_CHECK(q_out.is_contiguous() && q_out.numel() == n * Hq * D, op,
+              ": q_out must be a contiguous [n, Hq, D] tensor");
+  TORCH_CHECK(pos.scalar_type() == at::kLong && pos.is_contiguous() &&
                   (seq ? seq->scalar_type() == at::kInt && seq->is_contiguous() &&
                              seq->numel() == n
                        : n <= cache_k.size(0)),
-              "laprune::qk_rope_append: int64 positions and int32 sequences, one per token");
+              op, ": int64 positions and int32 sequences, one per token");
   for (const at::Tensor* w : {opt(q_weight), opt(k_weight)})
-    TORCH_CHECK(!w || (w->scalar_type() == dt && w->is_contiguous() && w->numel() == D),
-                "laprune::qk_rope_append: norm weights [D] of the tensors' dtype");
+    TORCH_CHECK(!w || (w->scalar_type() == dt && w->is_contiguous() && w->numel() == D), op,
+                ": norm weights [D] of the cache dtype");
   const c10::DeviceGuard guard(q.device());
-  check(lap_qk_rope_append(ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1),
-                           ptr(v), v.stride(0), v.stride(1), ptr(cos), ptr(sin),
-                           n < 2 ? 0 : cos.stride(0), ptr(q_weight), (float)q_eps, ptr(k_weight),
-                           (float)k_eps, dtype_code(q), n, (int)cache_k.size(0), (int)Hq,
-                           (int)Hkv, (int)D, static_cast<const int32_t*>(ptr(seq)),
+  check(lap_qk_rope_append(ptr(q), q_st, D, ptr(k), k_st, D, ptr(v), v_st, D, ptr(cos), ptr(sin),
+                           cs_st, ptr(q_weight), (float)q_eps, ptr(k_weight), (float)k_eps,
+                           dtype_code(q), n, (int)cache_k.size(0), (int)Hq, (int)Hkv, (int)D,
+                           static_cast<const int32_t*>(ptr(seq)),
                            static_cast<const int64_t*>(ptr(pos)), ptr(cache_k),
                            cache_k.stride(0), cache_k.stride(1), cache_k.stride(2), ptr(cache_v),
                            cache_v.stride(0), cache_v.stride(1), cache_v.stride(2),
@@ -426,9 +443,8 @@ void check_cache(const char* op, const at::Tensor& q, const at::Tensor& keys,
 // tiles given: q, out [n, Hq, D] packed; none: q, out [B, Tq, Hq, D].
 void prompt_attention(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& vals,
                       const std::optional<at::Tensor>& tiles, int64_t tokens_per_tile,
-                      int64_t nsplit, int64_t max_keys, double scale, const at::Tensor& out,
-                      const std::optional<at::Tensor>& ws) {
-  same_gpu("laprune::prompt_attention", {&q, &keys, &vals, opt(tiles), &out, opt(ws)});
+                      int64_t nsplit, int64_t max_keys, double scale, const at::Tensor& out) {
+  same_gpu("laprune::prompt_attention", {&q, &keys, &vals, opt(tiles), &out});
   TORCH_CHECK(q.dim() == (tiles ? 3 : 4),
               "laprune::prompt_attention: q [n, Hq, D] with tiles, [B, Tq, Hq, D] without");
   check_cache("laprune::prompt_attention", q, keys, vals);
@@ -438,10 +454,19 @@ void prompt_attention(const at::Tensor& q, const at::Tensor& keys, const at::Ten
   TORCH_CHECK(!tiles || (tiles->scalar_type() == at::kInt && tiles->is_contiguous() &&
                          tiles->dim() == 2 && tiles->size(1) == 4 && tiles->size(0) <= INT32_MAX),
               "laprune::prompt_attention: tiles int32 [n, 4]");
-  TORCH_CHECK(!ws || ws->is_contiguous(), "laprune::prompt_attention: contiguous workspace");
   const int t = tiles ? 0 : 1;  // the token dimension
-  TORCH_CHECK(q.size(t) <= INT32_MAX, "laprune::prompt_attention: too many tokens");
+  TORCH_CHECK(q.size(t) <= INT32_MAX && nsplit <= 1024,
+              "laprune::prompt_attention: too many tokens or splits");
   const c10::DeviceGuard guard(q.device());
+  std::optional<at::Tensor> ws;
+  if (nsplit > 1) {
+    size_t need = 0;
+    check(lap_prompt_attention_workspace_size(q.size(t) * (tiles ? 1 : q.size(0)),
+                                              (int)q.size(t + 1), (int)q.size(-1), (int)nsplit,
+                                              &need),
+          "lap_prompt_attention_workspace_size");
+    ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+  }
   check(lap_prompt_attention(
             ptr(q), tiles ? 0 : q.stride(0), q.stride(t), q.stride(t + 1), ptr(keys), ptr(vals),
             keys.stride(0), keys.stride(1), keys.stride(2), vals.stride(0), vals.stride(1),
@@ -450,33 +475,40 @@ void prompt_attention(const at::Tensor& q, const at::Tensor& keys, const at::Ten
             static_cast<const int32_t*>(ptr(tiles)), tiles ? (int)tiles->size(0) : 0,
             (int)tokens_per_tile, (int)nsplit, (int)max_keys, (float)scale, ptr(out),
             tiles ? 0 : out.stride(0), out.stride(t), out.stride(t + 1), ptr(ws),
-            ws ? (size_t)ws->numel() * ws->element_size() : 0, stream_of(q)),
+            ws ? (size_t)ws->numel() : 0, stream_of(q)),
         "lap_prompt_attention");
 }
 
-void shared_decode(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& vals,
+// q [B, Hq, D] or [B, Hq, 1, D]; keys [0, T) of the caches.  The workspace's size goes by
+// the prefix and the keys, so a call takes it from the allocator (a captured graph keeps
+// its own).
+void shared_decode(const at::Tensor& q, const at::Tensor& keys, const at::Tensor& vals, int64_t T,
                    int64_t prefix, const std::optional<at::Tensor>& plans, double scale,
-                   const at::Tensor& out, const std::optional<at::Tensor>& ws) {
-  same_gpu("laprune::shared_decode", {&q, &keys, &vals, opt(plans), &out, opt(ws)});
-  TORCH_CHECK(q.dim() == 3, "laprune::shared_decode: q [B, Hq, D]");
-  check_cache("laprune::shared_decode", q, keys, vals);
+                   const at::Tensor& out) {
+  const char* op = "laprune::shared_decode";
+  same_gpu(op, {&q, &keys, &vals, opt(plans), &out});
+  TORCH_CHECK(q.dim() == 3 || (q.dim() == 4 && q.size(2) == 1), op, ": q [B, Hq, D]");
+  check_cache(op, q, keys, vals);
   TORCH_CHECK(keys.size(0) == q.size(0) && out.is_contiguous() &&
-                  out.scalar_type() == q.scalar_type() && out.numel() >= q.numel(),
-              "laprune::shared_decode: as many sequences as keys, out like q");
+                  out.scalar_type() == q.scalar_type() && out.numel() == q.numel(),
+              op, ": as many sequences as keys, out like q");
   TORCH_CHECK(!plans || (plans->scalar_type() == at::kInt && plans->is_contiguous() &&
                          plans->numel() >= q.size(0) * 8),
-              "laprune::shared_decode: plans must hold B lap_row_plan records");
-  TORCH_CHECK(!ws || ws->is_contiguous(), "laprune::shared_decode: contiguous workspace");
-  TORCH_CHECK(prefix >= 0 && prefix <= keys.size(2),
-              "laprune::shared_decode: the prefix exceeds the keys");
+              op, ": plans must hold B lap_row_plan records");
+  TORCH_CHECK(T <= keys.size(2), op, ": ", T, " keys of ", keys.size(2), " rows");
+  TORCH_CHECK(prefix >= 0 && prefix <= T, op, ": a prefix of ", prefix, " of ", T, " keys");
+  const int B = (int)q.size(0), Hq = (int)q.size(1), Hkv = (int)keys.size(1), D = (int)q.size(-1);
   const c10::DeviceGuard guard(q.device());
+  size_t need = 0;
+  check(lap_shared_attn_decode_workspace_size(B, Hq, Hkv, D, (int)T, (int)prefix, &need),
+        "lap_shared_attn_decode_workspace_size");
+  const at::Tensor ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
   check(lap_shared_attn_decode(ptr(q), q.stride(0), q.stride(1), ptr(keys), ptr(vals),
-                               dtype_code(q), (int)q.size(0), (int)q.size(1), (int)keys.size(1),
-                               (int)keys.size(2), (int)q.size(2), keys.stride(0), keys.stride(1),
-                               keys.stride(2), vals.stride(0), vals.stride(1), vals.stride(2),
-                               (int)prefix, static_cast<const lap_row_plan*>(ptr(plans)),
-                               (float)scale, ptr(out), ptr(ws),
-                               ws ? (size_t)ws->numel() * ws->element_size() : 0, stream_of(q)),
+                               dtype_code(q), B, Hq, Hkv, (int)T, D, keys.stride(0),
+                               keys.stride(1), keys.stride(2), vals.stride(0), vals.stride(1),
+                               vals.stride(2), (int)prefix,
+                               static_cast<const lap_row_plan*>(ptr(plans)), (float)scale,
+                               ptr(out), ptr(ws), need, stream_of(q)),
         "lap_shared_attn_decode");
 }
 
@@ -506,15 +538,14 @@ TORCH_LIBRARY(laprune, m) {
   m.def("rope_tables(Tensor pos, Tensor inv_freq, float scaling, Tensor(a!) cos, "
         "Tensor(b!) sin) -> ()");
   m.def("pack_prompts(Tensor new_lens, Tensor? cached, int total, int tokens_per_tile, "
-        "Tensor(a!) starts, Tensor(b!) seq, Tensor(c!) pos, Tensor(d!)? tiles) -> ()");
+        "int n_tiles) -> (Tensor starts, Tensor seq, Tensor pos, Tensor? tiles)");
   m.def("qk_rope_append(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor? q_weight, "
         "float q_eps, Tensor? k_weight, float k_eps, Tensor? seq, Tensor pos, "
         "Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor(c!) q_out) -> ()");
   m.def("prompt_attention(Tensor q, Tensor keys, Tensor vals, Tensor? tiles, "
-        "int tokens_per_tile, int nsplit, int max_keys, float scale, Tensor(a!) out, "
-        "Tensor(b!)? ws) -> ()");
-  m.def("shared_decode(Tensor q, Tensor keys, Tensor vals, int prefix, Tensor? plans, "
-        "float scale, Tensor(a!) out, Tensor(b!)? ws) -> ()");
+        "int tokens_per_tile, int nsplit, int max_keys, float scale, Tensor(a!) out) -> ()");
+  m.def("shared_decode(Tensor q, Tensor keys, Tensor vals, int T, int prefix, Tensor? plans, "
+        "float scale, Tensor(a!) out) -> ()");
   m.def("argmax_rows(Tensor x, Tensor(a!) out, Tensor(b!)? copy=None) -> ()");
 }
 

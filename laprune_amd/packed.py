@@ -75,7 +75,7 @@ def pack_prompts(lens, cached=None, total: int | None = None, max_keys: int | No
             raise ValueError("pack_prompts: tensor lengths need total, and max_keys with cached ones")
         if lens.dtype != torch.int32 or lens.dim() != 1 or lens.numel() == 0:
             raise ValueError("pack_prompts: lengths must be an int32 tensor [B]")
-        B, dev = lens.numel(), lens.device
+        B = lens.numel()
         host = None, None
         new_dev, cached_dev = lens, cached
         if max_keys is None:
@@ -103,7 +103,7 @@ def pack_prompts(lens, cached=None, total: int | None = None, max_keys: int | No
         new_dev, cached_dev = both[0], both[1]
     if total < 0 or max_keys < 0:
         raise ValueError("pack_prompts: negative total or max_keys")
-    heads = shape = tiles = None
+    heads = shape = None
     if (num_q_heads, num_kv_heads, head_dim) != (None, None, None):
         if None in (num_q_heads, num_kv_heads, head_dim):
             raise ValueError("pack_prompts: num_q_heads, num_kv_heads and head_dim go together")
@@ -112,9 +112,6 @@ def pack_prompts(lens, cached=None, total: int | None = None, max_keys: int | No
         if host[0] is not None:
             n = sum(-(-t // shape[0]) for t in host[0])
             shape = prompt_shape(total, B, max_keys, *heads, n)
-        tiles = torch.empty((shape[1], 4), dtype=torch.int32, device=dev)
-    starts = torch.empty(B + 1, dtype=torch.int32, device=dev)
-    seq = torch.empty(total, dtype=torch.int32, device=dev)
-    pos = torch.empty(total, dtype=torch.int64, device=dev)
-    ops().pack_prompts(new_dev, cached_dev, total, shape[0] if shape else 1, starts, seq, pos, tiles)
+    bt, n_tiles, _ = shape or (1, -1, 1)
+    starts, seq, pos, tiles = ops().pack_prompts(new_dev, cached_dev, total, bt, n_tiles)
     return PackedPrompts(B, total, max_keys, heads, shape, starts, seq, pos, tiles, *host)

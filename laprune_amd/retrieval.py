@@ -426,47 +426,40 @@ class DenseDecoder:
         shared_prefix: the first so many tokens are the same in every sequence;
         their rows of sequence 0 are read once for the whole batch, and the other
         sequences' copies not at all."""
-        if q.dim() == 4:
-            q = q[:, :, 0, :]
-        B, Hq, Hkv, D = self.B, self.Hq, self.Hkv, self.D
+        B, Hkv, D = self.B, self.Hkv, self.D
         T = keys.shape[2]
         rows = _per_row(lengths, B, "lengths")
+        pdev = None
         if rows is not None and (len(set(rows)) > 1 or rows[0] != T):
             if max(rows) > T or min(rows) < 1:
                 raise RuntimeError("lengths must lie in [1, keys.shape[2]]")
-            if shared_prefix > min(rows):
-                raise RuntimeError(f"a shared prefix of {shared_prefix} tokens exceeds a "
-                                   f"sequence of {min(rows)}")
             if self._plans is None:
                 self._plans = PlanBuffer(B, q.device)
             if tuple(rows) != self._plan_key:
                 self._plans.upload([(t, t, 0, 0, 0, 0, 0, t) for t in rows])
                 self._plan_key = tuple(rows)
             pdev = self._plans.dev
-            if shared_prefix:
-                return self._shared(q, keys[:, :, :max(rows)], vals[:, :, :max(rows)],
-                                    shared_prefix, pdev)
-            self._ops.attn_decode_ragged(q, keys, vals, None, Hkv, 0, pdev, 0, max(rows),
-                                         1.0 / math.sqrt(D), self.out, self.ws)
-            return self.out.unsqueeze(2)
+            T = max(rows)
         if shared_prefix:
-            if shared_prefix > T:
-                raise RuntimeError(f"a shared prefix of {shared_prefix} tokens exceeds {T} keys")
-            return self._shared(q, keys, vals, shared_prefix, None)
-        return self._dense_uniform(q, keys, vals)
+            if shared_prefix > (T if pdev is None else min(rows)):
+                raise RuntimeError(f"a shared prefix of {shared_prefix} tokens exceeds a sequence "
+                                   f"of {T if pdev is None else min(rows)}")
+            return self._shared(q, keys, vals, T, shared_prefix, pdev)
+        if q.dim() == 4:
+            q = q[:, :, 0, :]
+        if pdev is None:
+            return self._dense_uniform(q, keys, vals)
+        self._ops.attn_decode_ragged(q, keys, vals, None, Hkv, 0, pdev, 0, T,
+                                     1.0 / math.sqrt(D), self.out, self.ws)
+        return self.out.unsqueeze(2)
 
-    def _shared(self, q, keys, vals, prefix: int, plans) -> torch.Tensor:
-        B, Hq, Hkv, D = self.B, self.Hq, self.Hkv, self.D
-        if prefix < 0 or q.shape != (B, Hq, D) or keys.shape[1] != Hkv:
+    def _shared(self, q, keys, vals, T: int, prefix: int, plans) -> torch.Tensor:
+        if prefix < 0 or q.numel() != self.out.numel() or keys.shape[1] != self.Hkv:
             raise RuntimeError("shared-prefix step: a prefix of at least 0 tokens and tensors of "
                                "the decoder's geometry expected")
-        if q.data_ptr() % 16 or q.stride(2) != 1 or any(s % 8 for s in q.stride()[:2]):
+        if q.data_ptr() % 16 or q.stride(-1) != 1 or q.stride(0) % 8 or q.stride(1) % 8:
             q = q.contiguous()
-        need = N.size_query("lap_shared_attn_decode_workspace_size", B, Hq, Hkv, D, keys.shape[2],
-                            prefix)
-        # its size goes by the prefix and the keys; a captured graph keeps its own
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        self._ops.shared_decode(q, keys, vals, prefix, plans, 1.0 / math.sqrt(D), self.out, ws)
+        self._ops.shared_decode(q, keys, vals, T, prefix, plans, 1.0 / math.sqrt(self.D), self.out)
         return self.out.unsqueeze(2)
 
     @torch.no_grad()
@@ -475,10 +468,10 @@ class DenseDecoder:
         """Dense decode with each sequence's length read from device plans
         (t_total, tail [0, t_total)); fixed launch arguments, as
         SparseDecoder.step_dev.  shared_prefix as in :meth:`step`."""
+        if shared_prefix:
+            return self._shared(q, keys, vals, keys.shape[2], shared_prefix, plans)
         if q.dim() == 4:
             q = q[:, :, 0, :]
-        if shared_prefix:
-            return self._shared(q, keys, vals, shared_prefix, plans)
         B, Hq, Hkv, D = self.B, self.Hq, self.Hkv, self.D
         T = keys.shape[2]
         self._ops.attn_decode_ragged(q, keys, vals, None, Hkv, 0, plans, 0, T,

@@ -238,9 +238,9 @@ def test_every_tile_shape_and_split(dev, dtype, rows, nsplit, D):
     bt = rows // 3
     shape = (bt, sum(lens) // bt + len(lens), nsplit)
     plan = packed.pack_prompts(lens, cached, device=dev, num_q_heads=Hq, num_kv_heads=Hkv, head_dim=D)
-    plan.shape, plan.tiles = shape, torch.empty((shape[1], 4), dtype=torch.int32, device=dev)
     both = torch.tensor([lens, cached], dtype=torch.int32, device=dev)
-    packed.ops().pack_prompts(both[0], both[1], plan.total, bt, plan.starts, plan.seq, plan.pos, plan.tiles)
+    plan.shape = shape
+    plan.tiles = packed.ops().pack_prompts(both[0], both[1], plan.total, bt, shape[1])[3]
     out = torch.full((plan.total + 5, Hq, D), 3.0, dtype=dtype, device=dev)
     prompt_attention(q, k, v, plan, out=out[:plan.total])
     _check_prompt(out[:plan.total], q, k, v, lens, cached)
@@ -468,10 +468,10 @@ def test_refusals_on_the_gpu(dev):
     bad(x, k, v, plan, match="aligned")
     with pytest.raises(RuntimeError, match="tile"):
         from laprune_amd._ops import ops
-        ops().prompt_attention(q, k, v, plan.tiles, 65, 1, 10, 0.1, torch.empty_like(q), None)
+        ops().prompt_attention(q, k, v, plan.tiles, 65, 1, 10, 0.1, torch.empty_like(q))
     c = _cache(dev, torch.bfloat16, 1, 2, 64, 16)
     rq, rk, rv, cos, sin, _ = _rope_inputs(dev, torch.bfloat16, 10, 4, 2, 64)
-    with pytest.raises(RuntimeError, match="tokens expected"):
+    with pytest.raises(RuntimeError, match="10 tokens expected"):
         c.rope_append_packed(rq[:, :9], rk, rv, cos, sin, plan)
     with pytest.raises(RuntimeError, match="cache dtype"):
         c.rope_append_packed(rq.half(), rk, rv, cos, sin, plan)
