@@ -324,6 +324,21 @@ class DecodeKVCache:
         self._encode_rows([b for b in range(self.B) if plan.lens[b]], True, None)
         return q_out
 
+    def append_step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+                    sin: torch.Tensor, pos: torch.Tensor, q_norm: tuple | None = None,
+                    k_norm: tuple | None = None) -> torch.Tensor:
+        """:meth:`rope_append` of one token behind every sequence's cached ones (pos
+        [B, 1], their lengths), growing the buffers when needed, and the encode that the
+        policy says to.  Returns the rotated query [B, Hq, 1, D]."""
+        ends = [n + 1 for n in self.lengths]
+        if max(ends) > self.capacity:
+            self._grow(max(ends))
+        q_out = q.new_empty((self.B, q.shape[-1] // self.D, self.D))
+        q_out = self.rope_append(q, k, v, cos, sin, pos, q_out, q_norm, k_norm)
+        self.lengths = ends
+        self.encode()
+        return q_out
+
     def encode_ranges(self, ranges: torch.Tensor) -> None:
         """Encode each sequence's device range ([B, 2] int32, at most
         group_size tokens; empty ranges cost a workgroup exit)."""

@@ -10,12 +10,16 @@ Mirrors the reference's model plumbing for the decode path:
   * ``AQGeneration.generate`` (aq_generation.py:114-151): prefill all prompt
     tokens but the last, then greedy decode one token at a time.
 
-Each layer owns a :class:`~laprune_amd.cache.DecodeKVCache`; LAPrune layers
-decode through :class:`~laprune_amd.retrieval.SparseDecoder` (LUT -> fused
+Each layer owns a :class:`~laprune_amd.cache.DecodeKVCache`; prompts run through the
+packed kernels (rotation and cache write in one launch, causal attention over the
+caches); LAPrune layers decode through :class:`~laprune_amd.retrieval.SparseDecoder` (LUT -> fused
 score -> top-k -> sparse attention, all HIP), dense layers through
 :class:`~laprune_amd.retrieval.DenseDecoder`.  Sequences of one batch may have
-different lengths (ragged): prefill them one row at a time with
-:meth:`LAPruneLlama.prefill_row`, then decode the batch together.
+different lengths (ragged): prefill them in one pass with
+:meth:`LAPruneLlama.prefill_packed` or one at a time with
+:meth:`LAPruneLlama.prefill_row`, whole or in pieces, then decode the batch together.
+Prompts that begin alike: :meth:`LAPruneLlama.prefill_shared` runs the common part once,
+and the dense layers' steps read it once for the batch.
 
 The model is a plain ``transformers`` ``LlamaForCausalLM``; nothing here
 downloads anything (build it from a local ``LlamaConfig``).
@@ -32,7 +36,9 @@ import torch.nn.functional as F
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from ._ops import ops, unwatched
+from .attention import prompt_attention
 from .cache import DecodeKVCache
+from .packed import pack_prompts
 from .retrieval import DenseDecoder, RetrievalConfig, SparseDecoder, check_step_health
 
 
@@ -159,6 +165,12 @@ del _f
 
 
 @functools.lru_cache(None)
+def _llama_norm() -> type:
+    from transformers.models.llama.modeling_llama import LlamaRMSNorm
+    return LlamaRMSNorm
+
+
+@functools.lru_cache(None)
 def _silu_types() -> tuple:
     from transformers.activations import ACT2FN
     return torch.nn.SiLU, type(ACT2FN["silu"])
@@ -272,7 +284,10 @@ class LAPruneLlama:
             attn.forward = self._make_forward(i, attn)
         _fuse_decode_ops(model)
         self._mask = _step_mask(model, batch, self.dev)
-        self._row = None  # sequence being prefilled alone (ragged prefill)
+        self._plan = None    # tables of the packed prompts being prefilled
+        self._row = None     # sequence being prefilled alone without them
+        self._pos = None     # positions of the eager step being run
+        self.shared_prefix = 0  # tokens that every sequence begins with (prefill_shared)
         self.health_every = health_every
         self._since_check = 0
         self._dev_mode = False
@@ -341,31 +356,63 @@ class LAPruneLlama:
             return self._attention(idx, attn, hidden_states, position_embeddings)
         return forward
 
+    def _head_norms(self, attn, q, k, fuse: bool):
+        """The layer's norms of q's and k's heads, where it has them: q and k as they are
+        and the (weight, eps) of each for the rotation's kernel (``fuse``), or its
+        module's output and None (also for a norm that is not the stock one)."""
+        out = []
+        for mod, x in ((getattr(attn, "q_norm", None), q), (getattr(attn, "k_norm", None), k)):
+            w = getattr(mod, "weight", None)
+            if mod is None:
+                out.append((x, None))
+            elif (fuse and type(mod) is _llama_norm() and w.numel() == self.D and w.dtype == x.dtype and
+                  w.device == x.device and self.D % 16 == 0 and _plain_tensor(w) and _unhooked(mod)):
+                out.append((x, (w, mod.variance_epsilon)))
+            else:
+                out.append((mod(x.unflatten(-1, (-1, self.D))).flatten(-2), None))
+        (q, qn), (k, kn) = out
+        return q, k, dict(q_norm=qn, k_norm=kn)
+
+    def _shares(self) -> int:
+        """The shared prefix that a dense step reads once (0: nothing to share, or so little
+        that one launch more costs as much: 64 tokens of 4 sequences, own and shared, 9.6
+        and 10.0 us, of 64 sequences 17.4 and 20.9; 256 tokens 10.1 and 9.7, 24.5 and
+        20.8; 4096 tokens 20.6 and 12.3, 202 and 31)."""
+        return self.shared_prefix if self.B > 1 and self.shared_prefix >= 128 else 0
+
     def _attention(self, idx, attn, h, position_embeddings):
         B, T, _ = h.shape
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
         cos, sin = position_embeddings
         st = self.states[idx]
+        qp, kp, vp = self._project(attn, h)
+        qp, kp, norms = self._head_norms(attn, qp, kp, T == 1 or self._plan is not None)
+        if self._plan is not None:
+            q = st.cache.append_packed(qp, kp, vp, cos, sin, self._plan, **norms)
+            o = prompt_attention(q, st.cache.k, st.cache.v, self._plan)
+            return attn.o_proj(o.view(B, T, Hq * D)), None
         if T == 1 and self._dev_mode:
             # fixed launches, every per-step value in device memory; RoPE and
             # the cache write are one kernel
-            qp, kp, vp = self._project(attn, h)
-            q = st.cache.rope_append(qp, kp, vp, cos, sin, self._g_pos, self._q_rope)
+            q = st.cache.rope_append(qp, kp, vp, cos, sin, self._g_pos, self._q_rope, **norms)
             if st.sparse is not None:
                 if self._g_flush:
                     st.cache.encode_ranges(self._g_ranges)
                 o = st.sparse.step_dev(q, st.cache.codes, st.cache.k, st.cache.v,
                                        self._g_plan_sparse)
             else:
-                o = st.dense.step_dev(q, st.cache.k, st.cache.v, self._g_plan_dense)
+                o = st.dense.step_dev(q, st.cache.k, st.cache.v, self._g_plan_dense,
+                                      shared_prefix=self._shares())
             o = o.transpose(1, 2).reshape(B, T, Hq * D)
             return attn.o_proj(o), None
-        qp, kp, vp = self._project(attn, h)
+        if T == 1 and (norms["q_norm"] or norms["k_norm"]):
+            q = st.cache.append_step(qp, kp, vp, cos, sin, self._pos, **norms)
+            return attn.o_proj(self._step(st, q).transpose(1, 2).reshape(B, T, Hq * D)), None
         q = qp.reshape(B, T, Hq, D).transpose(1, 2)
         k = kp.reshape(B, T, Hkv, D).transpose(1, 2)
         v = vp.reshape(B, T, Hkv, D).transpose(1, 2)
         q, k = self._rope(q, k, cos, sin)
-        if T > 1:  # prefill: causal attention over the prompt, encode all its keys
+        if T > 1:  # a prompt that the packed kernels do not serve
             if self._row is None:
                 if any(n != 0 for n in st.cache.lengths):
                     raise RuntimeError("batched prefill needs empty caches (use reset())")
@@ -383,12 +430,15 @@ class LAPruneLlama:
             if self._row is not None:
                 raise RuntimeError("single-token steps decode the whole batch")
             st.cache.append(k, v)  # encodes each sequence's 64-token groups
-            if st.sparse is not None:
-                o = st.sparse.step_cached(q, st.cache)
-            else:
-                o = st.dense.step(q, st.cache.k, st.cache.v, lengths=st.cache.lengths)
+            o = self._step(st, q)
         o = o.transpose(1, 2).reshape(B, T, Hq * D)
         return attn.o_proj(o), None
+
+    def _step(self, st, q):
+        if st.sparse is not None:
+            return st.sparse.step_cached(q, st.cache)
+        return st.dense.step(q, st.cache.k, st.cache.v, lengths=st.cache.lengths,
+                             shared_prefix=self._shares())
 
     # ------------------------------------------------------------ model calls
     def reset(self) -> None:
@@ -396,6 +446,7 @@ class LAPruneLlama:
         for st in self.states:
             st.cache.lengths = [0] * self.B
             st.cache.encoded_lens = [0] * self.B
+        self.shared_prefix = 0
 
     @property
     def lengths(self) -> list[int]:
@@ -408,16 +459,46 @@ class LAPruneLlama:
         the layers' caches stay consistent."""
         lens = self.lengths
         rows = range(self.B) if rows is None else rows
-        need = max(lens[b] for b in rows) + new
+        new = [new] * len(rows) if isinstance(new, int) else new
+        need = max(lens[b] + n for b, n in zip(rows, new))
         if need > self.capacity:
             raise RuntimeError(f"{need} tokens exceed the capacity of {self.capacity} the "
                                "model was wrapped with (wrap it with a larger capacity)")
 
-    def _forward(self, ids: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
-        mask = self._mask if ids.shape[1] == 1 else None
+    def _forward(self, ids: torch.Tensor, pos: torch.Tensor, keep=1) -> torch.Tensor:
+        # every layer's attention ignores the mask (a packed pass would have one of its
+        # whole length squared built from the positions)
+        mask = self._mask
+        if mask is not None:
+            mask = mask[:ids.shape[0]] if ids.shape[1] == 1 or self._plan is not None else None
         out = self.model(input_ids=ids, attention_mask=mask, position_ids=pos, use_cache=False,
-                         logits_to_keep=1)
-        return out.logits[:, -1]
+                         logits_to_keep=keep)
+        return out.logits[:, -1] if isinstance(keep, int) else out.logits[0]
+
+    def _packs(self) -> bool:
+        """Whether the packed prompt kernels serve this model."""
+        return self.D in (64, 128, 256) and self.Hq // self.Hkv <= 128
+
+    def _prefill(self, rows: list[int], prompts: list[torch.Tensor]) -> torch.Tensor:
+        """One packed pass: prompts[i] behind what sequence rows[i] has cached; its last
+        position's logits [len(rows), V]."""
+        new = [int(p.numel()) for p in prompts]
+        if not new or min(new) < 1:
+            raise RuntimeError("a prompt needs at least one token")
+        self._check_room(new, rows)
+        lens = [0] * self.B
+        for b, n in zip(rows, new):
+            lens[b] = n
+        # packed in the order of the sequences
+        order = sorted(range(len(rows)), key=lambda i: rows[i])
+        ids = torch.cat([prompts[i].reshape(-1).to(self.dev) for i in order])[None]
+        ends = torch.tensor([sum(lens[:b + 1]) - 1 for b in rows]).to(self.dev)
+        self._plan = pack_prompts(lens, self.lengths, device=self.dev, num_q_heads=self.Hq,
+                                  num_kv_heads=self.Hkv, head_dim=self.D)
+        try:
+            return self._forward(ids, self._plan.pos[None], ends)
+        finally:
+            self._plan = None
 
     @torch.no_grad()
     def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
@@ -428,16 +509,25 @@ class LAPruneLlama:
         if any(n != 0 for n in self.lengths):
             raise RuntimeError("batched prefill needs empty caches (use reset())")
         self._check_room(T)
+        if T > 1 and self._packs():
+            return self._prefill(list(range(self.B)), list(input_ids))
         pos = torch.arange(T, device=self.dev)[None].expand(self.B, T)
+        self._pos = pos
         return self._forward(input_ids.to(self.dev), pos)
 
     @torch.no_grad()
     def prefill_row(self, b: int, input_ids: torch.Tensor) -> torch.Tensor:
-        """Prefill sequence b alone ([1, T_b] prompt); returns its logits [1, V]."""
+        """Prefill sequence b alone ([1, T_b] prompt), behind what it has cached (a long
+        prompt may come in pieces); returns its logits [1, V]."""
+        if self._packs():
+            return self.prefill_packed([input_ids], [b])
         T = input_ids.shape[-1]
         if not 0 <= b < self.B:
             raise RuntimeError(f"sequence {b} out of range for batch {self.B}")
         self._check_room(T, rows=[b])
+        if self.lengths[b]:
+            raise RuntimeError("a prompt in pieces needs the packed prompt kernels (head dim 64, "
+                               "128 or 256)")
         self._row = b
         try:
             pos = torch.arange(T, device=self.dev)[None]
@@ -446,10 +536,46 @@ class LAPruneLlama:
             self._row = None
 
     @torch.no_grad()
+    def prefill_packed(self, prompts: list[torch.Tensor],
+                       rows: list[int] | None = None) -> torch.Tensor:
+        """Prefill prompts of different lengths in one pass: prompts[i] (ids [T_i] or
+        [1, T_i]) behind what sequence rows[i] has cached (by default sequence i).
+        Returns each prompt's last-position logits [len(prompts), V]."""
+        rows = list(range(len(prompts))) if rows is None else [int(b) for b in rows]
+        if len(rows) != len(prompts) or len(set(rows)) != len(rows):
+            raise RuntimeError("prefill_packed: one sequence of its own per prompt")
+        for b in rows:
+            if not 0 <= b < self.B:
+                raise RuntimeError(f"sequence {b} out of range for batch {self.B}")
+        if not self._packs():
+            raise RuntimeError("packed prompts need head dim 64, 128 or 256 and at most 128 query "
+                               "heads per KV head")
+        return self._prefill(rows, prompts)
+
+    @torch.no_grad()
+    def prefill_shared(self, input_ids: torch.Tensor) -> torch.Tensor:
+        """Prefill the tokens [1, P] that every sequence begins with: they run once, every
+        sequence's caches receive them, and dense layers' steps read them once for the
+        whole batch.  The sequences' own prompts follow (``prefill_packed``).  Returns
+        the last position's logits [1, V]."""
+        if any(n != 0 for n in self.lengths):
+            raise RuntimeError("a shared prefix needs empty caches (use reset())")
+        logits = self.prefill_packed([input_ids], [0])
+        P = self.lengths[0]
+        for st in self.states:
+            c = st.cache
+            for x in (c.k, c.v, c.codes):
+                x[1:, :, :P] = x[:1, :, :P]
+            c.lengths = [P] * self.B
+            c.encoded_lens = [c.encoded_lens[0]] * self.B
+        self.shared_prefix = P
+        return logits
+
+    @torch.no_grad()
     def decode(self, tokens: torch.Tensor) -> torch.Tensor:
         """One decode step for all sequences: tokens [B, 1]; returns logits [B, V]."""
         self._check_room(1)
-        pos = torch.tensor(self.lengths, device=self.dev)[:, None]
+        pos = self._pos = torch.tensor(self.lengths, device=self.dev)[:, None]
         logits = self._forward(tokens.reshape(self.B, 1).to(self.dev), pos)
         self._count_step()
         return logits
@@ -570,10 +696,11 @@ class LAPruneLlama:
         else:
             self._g_tok.copy_(self._g_next)
         self._upload_step()
-        sig = tuple((st.cache.k.data_ptr(), st.cache.v.data_ptr(), st.cache.codes.data_ptr())
-                    for st in self.states)
+        sig = (self._shares(),
+               *((st.cache.k.data_ptr(), st.cache.v.data_ptr(), st.cache.codes.data_ptr())
+                 for st in self.states))
         if self._graph is not None and sig != self._graph_sig:
-            self._graph = None  # a cache was reallocated (grown): capture again
+            self._graph = None  # a cache was reallocated (grown), or another prefix: capture again
         if self._graph is None:
             self._graph = {}
             self._graph_sig = sig
