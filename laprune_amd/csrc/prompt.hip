@@ -787,8 +787,9 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
   LAP_CHECK(tokens_per_tile > 0 && (int64_t)tokens_per_tile * G <= kRows && nsplit > 0 &&
                 n_tiles >= 0 && max_keys >= 0,
             "lap_prompt_attention: bad tile shape");
-  if (!tiles) n_tiles = B * ((Tq + tokens_per_tile - 1) / tokens_per_tile);
-  if (n_tiles == 0) return LAP_OK;
+  const int tps = (Tq - 1) / tokens_per_tile + 1;
+  const int64_t all_tiles = tiles ? n_tiles : (int64_t)B * tps;
+  if (all_tiles == 0) return LAP_OK;
   FlashArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
@@ -799,15 +800,17 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = G; a.Tq = Tq; a.Tk = Tk;
   a.tiles = reinterpret_cast<const int4*>(tiles);
   a.bt = tokens_per_tile;
-  a.tps = (Tq + tokens_per_tile - 1) / tokens_per_tile;
+  a.tps = tps;
   a.nsplit = nsplit;
-  a.per_split = (std::max(1, (std::min(max_keys, Tk) + nsplit - 1) / nsplit) + kGran - 1) / kGran * kGran;
+  a.per_split =
+      (std::max(1, (int)(((int64_t)std::min(max_keys, Tk) + nsplit - 1) / nsplit)) + kGran - 1) /
+      kGran * kGran;
   a.c = scale * kLog2e;
   a.out = static_cast<uint16_t*>(out);
   a.o_sb = o_sb; a.o_st = o_st; a.o_sh = o_sh;
   const int64_t rows = (int64_t)(tiles ? 1 : B) * Tq * Hq;
-  const int64_t grid = (int64_t)n_tiles * nsplit * Hkv;
-  LAP_CHECK(grid <= 0x7fffffff && (int64_t)n_tiles * tokens_per_tile * Hq <= 0x7fffffff,
+  const int64_t grid = all_tiles * nsplit * Hkv;
+  LAP_CHECK(grid <= 0x7fffffff && all_tiles * tokens_per_tile * Hq <= 0x7fffffff,
             "lap_prompt_attention: too many rows");
   if (nsplit > 1) {
     const size_t need = part_bytes(rows, nsplit, D);
@@ -817,7 +820,7 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
     a.part_ml = a.part_o + rows * nsplit * D;
   }
   return launch_by_type<false>(a, dtype, D, grid,
-                               (int64_t)n_tiles * tokens_per_tile * Hq, as_stream(stream));
+                               all_tiles * tokens_per_tile * Hq, as_stream(stream));
 }
 
 namespace lap {

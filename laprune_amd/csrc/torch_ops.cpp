@@ -371,11 +371,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, std::optional<at::Tensor>> pack_p
 int64_t token_stride(const char* op, const at::Tensor& x, int64_t n) {
   TORCH_CHECK(x.dim() >= 2 && x.numel() == n * x.size(-1) && x.stride(-1) == 1, op, ": rows of ",
               n, " tokens expected, each contiguous");
-  int64_t st = 0, next = 0;  // next: the stride an outer dimension must have
+  int64_t st = 0, next = -1;  // next: the stride an outer dimension must have
   for (int64_t d = x.dim() - 2; d >= 0; --d) {
     if (x.size(d) == 1) continue;
-    TORCH_CHECK(!next || x.stride(d) == next, op, ": tokens must lie at one stride");
-    if (!next) st = x.stride(d);
+    TORCH_CHECK(next < 0 || x.stride(d) == next, op, ": tokens must lie at one stride");
+    if (next < 0) st = x.stride(d);
     next = x.stride(d) * x.size(d);
   }
   return st;

@@ -155,6 +155,24 @@ def test_step_form_equals_the_packed_form(dev, dtype):
         assert torch.equal(qa, qb) and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
 
 
+def test_row_layouts(dev):
+    """Tokens in two dimensions of one stride, and one table row for all tokens; tokens
+    that do not lie at one stride are refused."""
+    from laprune_amd.packed import pack_prompts
+    Hq, Hkv, D = 4, 2, 64
+    q, k, v, cos, sin, _ = _rope_inputs(dev, torch.float16, 12, Hq, Hkv, D, seed=6)
+    plan = pack_prompts([6, 6], device=dev)
+    two = lambda x: x.unflatten(1, (2, 6))[0]
+    one = lambda x: x[:, :1].expand(1, 12, D)
+    a, b = _cache(dev, torch.float16, 2, Hkv, D, 8), _cache(dev, torch.float16, 2, Hkv, D, 8)
+    qa = a.rope_append_packed(two(q), two(k), two(v), one(cos), one(sin), plan)
+    qb = b.rope_append_packed(q, k, v, one(cos).contiguous(), one(sin).contiguous(), plan)
+    assert torch.equal(qa, qb) and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+    for bad in (two(cos)[:, :1].expand(2, 6, D), two(cos).transpose(0, 1)):
+        with pytest.raises(RuntimeError, match="one stride"):
+            a.rope_append_packed(q, k, v, bad, one(sin), plan)
+
+
 def test_tokens_of_no_sequence_and_past_the_capacity(dev):
     """Tokens behind the last sequence leave everything as it was; a token past the
     capacity is rotated but not cached."""
@@ -377,6 +395,8 @@ def test_do_sdpa_attn_of_prompts(dev, dtype, shape):
     assert not _prompt_kernel_fits(q2, k, v)
     do_sdpa_attn(q2, k, v, already_rope=True).float().sum().backward()
     assert q2.grad is not None
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert not _prompt_kernel_fits(q, k, v)
     odd = torch.empty(B * Hq * Tq * D + 1, dtype=dtype, device=dev)[1:].view(B, Hq, Tq, D)
     assert not _prompt_kernel_fits(odd, k, v)
 
