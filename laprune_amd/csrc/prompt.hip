@@ -18,6 +18,15 @@
 // All query heads of a KV head lie in one block (row = token * G + head): K and V are
 // read once for the group, and 32 rows span few tokens, so little of a causal block
 // is masked.  A wave skips a tile of keys that none of its rows sees.
+//
+// K and V tiles are copied straight into LDS, one tile ahead; 252 registers and 64 KB let
+// two workgroups share a CU, whose products and exponentials overlap.  One prompt of
+// 16384 tokens, 32 query heads on 8, D = 128: 2.07 ms, 1060 TFLOP/s, where a large library
+// product reaches 1280 to 1330 on the same card.  The matrix pipe is busy 58 % of the
+// cycles and the card runs at 1.77 GHz under this load: saved cycles come back as a lower
+// clock (20 % fewer cycles than an earlier form gave 9 % in time).  LDS reads have no bank
+// conflicts.  Short prompts wait: a tile takes one workgroup 1.2 us, its start, masked
+// tile and end together about 15 us of a 2048-token prompt's 55.
 #include "common.h"
 #include "attn_core.h"
 
