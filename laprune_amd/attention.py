@@ -79,7 +79,10 @@ def _prompt_kernel_fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bo
             q.shape[3] in (64, 128, 256) and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and
             q.shape[1] // k.shape[1] <= 128 and 0 < q.shape[2] <= k.shape[2] and
             all(type(t) in (torch.Tensor, torch.nn.Parameter) and _rows16(t) for t in (q, k, v)) and
-            k.shape[2] < 1 << 30 and max(k.stride(2), v.stride(2)) <= 1 << 24 and untraced() and
+            k.shape[2] < 1 << 30 and
+            # a launch takes less than 2^24 workgroups, each 128 // group tokens of a KV head
+            q.shape[0] * k.shape[1] * -(-q.shape[2] // (128 * k.shape[1] // q.shape[1])) < 1 << 24 and
+            max(k.stride(2), v.stride(2)) <= 1 << 24 and untraced() and
             not torch.is_autocast_enabled(q.device.type) and not _needs_grad(q, k, v))
 
 

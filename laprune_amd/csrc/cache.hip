@@ -296,7 +296,7 @@ extern "C" int lap_qk_rope_append(const void* q, int64_t q_st, int64_t q_sh, con
                static_cast<uint16_t*>(q_out)};
   const int lpr = D <= 16 ? 1 : D <= 32 ? 2 : D <= 64 ? 4 : D <= 128 ? 8 : 16;
   const int64_t blocks = (a.rows + 256 / lpr - 1) / (256 / lpr);
-  LAP_CHECK(blocks <= 0x7fffffff, "lap_qk_rope_append: too many rows");
+  LAP_CHECK(blocks <= kMaxBlocks256, "lap_qk_rope_append: too many rows");
   const dim3 grid((unsigned)blocks);
   hipStream_t st = as_stream(stream);
 #define LAP_QK_ROPE(DT)                                                                      \

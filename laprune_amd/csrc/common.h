@@ -18,6 +18,8 @@ namespace lap {
 // declaration order (t_codes, t_total, cand_start, cand_end, k, sink,
 // tail_start, tail_count).
 constexpr int kPlanInts = 8;
+// Workgroups of 256 threads that one launch takes: fewer than 2^32 work-items.
+constexpr int64_t kMaxBlocks256 = (1 << 24) - 1;
 static_assert(sizeof(lap_row_plan) == kPlanInts * sizeof(int32_t), "lap_row_plan layout");
 
 // ---------------------------------------------------------------- errors

@@ -681,9 +681,12 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(FlashArgs a
   merge_row<DT, D, WPR>(a, r, r < rows, a.out + (int64_t)r * D);
 }
 
+int merge_waves(int nsplit) { return nsplit > kMergeFew ? 4 : 1; }
+int64_t merge_blocks(int64_t rows, int nsplit) { return (rows * merge_waves(nsplit) + 3) / 4; }
+
 template <bool SHARED, int DT, int D, int WPR>
 void launch_merge(const FlashArgs& a, int64_t rows, hipStream_t st) {
-  const dim3 g((unsigned)((rows * WPR + 3) / 4)), threads(kMergeThreads);
+  const dim3 g((unsigned)merge_blocks(rows, a.nsplit)), threads(kMergeThreads);
   if constexpr (SHARED)
     hipLaunchKernelGGL((shared_merge_kernel<DT, D, WPR>), g, threads, 0, st, a, (int)rows);
   else hipLaunchKernelGGL((prompt_merge_kernel<DT, D, WPR>), g, threads, 0, st, a, (int)rows);
@@ -697,7 +700,7 @@ int launch_flash(const FlashArgs& a, int64_t grid, int64_t rows, hipStream_t st)
   else hipLaunchKernelGGL((prompt_kernel<DT, D>), g, dim3(kThreads), 0, st, a);
   LAP_LAUNCH_CHECK("attention of many rows");
   if (a.nsplit > 1) {
-    if (a.nsplit > kMergeFew) launch_merge<SHARED, DT, D, 4>(a, rows, st);
+    if (merge_waves(a.nsplit) == 4) launch_merge<SHARED, DT, D, 4>(a, rows, st);
     else launch_merge<SHARED, DT, D, 1>(a, rows, st);
     LAP_LAUNCH_CHECK("merge of splits");
   }
@@ -819,17 +822,20 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
   a.o_sb = o_sb; a.o_st = o_st; a.o_sh = o_sh;
   const int64_t rows = (int64_t)(tiles ? 1 : B) * Tq * Hq;
   const int64_t grid = all_tiles * nsplit * Hkv;
-  LAP_CHECK(grid <= 0x7fffffff && all_tiles * tokens_per_tile * Hq <= 0x7fffffff,
-            "lap_prompt_attention: too many rows");
+  LAP_CHECK(grid <= kMaxBlocks256, "lap_prompt_attention: too many rows");
+  const int64_t tile_rows = all_tiles * tokens_per_tile * Hq;  // at most 128 * grid
   if (nsplit > 1) {
+    LAP_CHECK(merge_blocks(tile_rows, nsplit) <= kMaxBlocks256,
+              "lap_prompt_attention: too many rows");
+    LAP_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+              "lap_prompt_attention: workspace must be 16-byte aligned");
     const size_t need = part_bytes(rows, nsplit, D);
     LAP_CHECK_CODE(workspace && workspace_bytes >= need, LAP_ERR_WORKSPACE,
                    "lap_prompt_attention: workspace of %zu bytes needed", need);
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + rows * nsplit * D;
   }
-  return launch_by_type<false>(a, dtype, D, grid,
-                               all_tiles * tokens_per_tile * Hq, as_stream(stream));
+  return launch_by_type<false>(a, dtype, D, grid, tile_rows, as_stream(stream));
 }
 
 namespace lap {
@@ -926,8 +932,11 @@ extern "C" int lap_shared_attn_decode(const void* q, int64_t q_sb, int64_t q_sh,
   const int64_t rows = (int64_t)B * Hq;
   const int64_t grid =
       ((int64_t)sh.pblocks * sh.psplit + (int64_t)B * (sh.nsplit - sh.psplit)) * Hkv;
-  LAP_CHECK(grid <= 0x7fffffff && rows <= 0x7fffffff, "lap_shared_attn_decode: too many rows");
+  LAP_CHECK(grid <= kMaxBlocks256 && merge_blocks(rows, sh.nsplit) <= kMaxBlocks256,
+            "lap_shared_attn_decode: too many rows");
   if (sh.nsplit > 1) {
+    LAP_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+              "lap_shared_attn_decode: workspace must be 16-byte aligned");
     const size_t need = part_bytes(rows, sh.nsplit, D);
     LAP_CHECK_CODE(workspace && workspace_bytes >= need, LAP_ERR_WORKSPACE,
                    "lap_shared_attn_decode: workspace of %zu bytes needed", need);

@@ -385,6 +385,8 @@ class LAPruneLlama:
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
         cos, sin = position_embeddings
         st = self.states[idx]
+        if T == 1 and self._row is not None:
+            raise RuntimeError("single-token steps decode the whole batch")
         qp, kp, vp = self._project(attn, h)
         qp, kp, norms = self._head_norms(attn, qp, kp, T == 1 or self._plan is not None)
         if self._plan is not None:
@@ -427,8 +429,6 @@ class LAPruneLlama:
                 o = F.scaled_dot_product_attention(q, kk, vv, is_causal=True,
                                                    scale=1.0 / math.sqrt(D))
         else:
-            if self._row is not None:
-                raise RuntimeError("single-token steps decode the whole batch")
             st.cache.append(k, v)  # encodes each sequence's 64-token groups
             o = self._step(st, q)
         o = o.transpose(1, 2).reshape(B, T, Hq * D)

@@ -501,3 +501,15 @@ def test_refusals_on_the_gpu(dev):
         c.rope_append_packed(rq, rk, rv, cos, sin, pack_prompts([5, 5], device=dev))
     with pytest.raises(RuntimeError, match="cached lengths"):
         c.append_packed(rq, rk, rv, cos, sin, pack_prompts([10], [3], device=dev))
+
+
+@pytest.mark.parametrize("Hq,Hkv,Tq", [(1, 1, 2), (4, 2, 65), (28, 4, 19), (128, 1, 3)])
+def test_batches_past_one_launch_keep_the_library(dev, Hq, Hkv, Tq):
+    """A launch takes fewer than 2^24 workgroups (nothing runs here: broadcast views)."""
+    from laprune_amd.attention import _prompt_kernel_fits
+    most = ((1 << 24) - 1) // (Hkv * -(-Tq // (128 // (Hq // Hkv))))
+    q = torch.zeros((1, Hq, Tq, 64), dtype=torch.bfloat16, device=dev)
+    k = torch.zeros((1, Hkv, Tq, 64), dtype=torch.bfloat16, device=dev)
+    for B, fits in [(most, True), (most + 1, False)]:
+        x, y = (t.expand(B, -1, -1, -1) for t in (q, k))
+        assert _prompt_kernel_fits(x, y, y) == fits

@@ -177,3 +177,13 @@ def test_refusals(dev):
         lm.prefill_shared(ids[None, :3])
     lm.prefill_row(1, ids[:5])
     assert lm.lengths == [60, 10]
+
+
+def test_one_token_prompt_without_the_packed_kernels(dev):
+    """Alone it is no decode step of the batch, with head norms as without."""
+    for norms in (False, True):
+        _, lm = _pair(dev, 1, norms=norms)
+        lm._packs = lambda: False
+        with pytest.raises(RuntimeError, match="whole batch"):
+            lm.prefill_row(0, _ids(dev, 1, 1)[None])
+        assert lm.lengths == [0] and lm._row is None

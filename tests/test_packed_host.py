@@ -109,6 +109,33 @@ def test_invalid_arguments_of_the_c_abi(lib):
     assert lib.lap_prompt_shape(1, 1, 0, 1, 8, 2, 96, C.byref(i), C.byref(i), C.byref(i)) == 2
 
 
+def test_launches_past_the_limit_are_refused(lib):
+    """A launch takes fewer than 2^32 work-items: 2^24 workgroups of 256."""
+    from laprune_amd import _native as N
+    al, odd, null = C.c_void_p(4096), C.c_void_p(4100), None  # never dereferenced
+
+    def prompt(tiles, nt, ns=1, ws=null, B=1, Hkv=2):
+        return lib.lap_prompt_attention(al, 1024, 256, 64, al, al, 4096, 2048, 64, 4096, 2048, 64, N.BF16,
+                                        B, 2 * Hkv, Hkv, 64, 1, 9, tiles, nt, 64, ns, 9, 0.1, al, 1024, 256,
+                                        64, ws, 1 << 62, null)
+
+    def shared(B, T, ws=al):
+        return lib.lap_shared_attn_decode(al, 1024, 64, al, al, N.BF16, B, 4, 2, T, 64, 4096, 2048, 64, 4096,
+                                          2048, 64, 0, null, 0.1, al, ws, 0, null)
+
+    def rope(n):
+        return lib.lap_qk_rope_append(al, 256, 64, al, 128, 64, al, 128, 64, al, al, 64, null, 0.0, null, 0.0,
+                                      N.BF16, n, 2, 4, 2, 64, al, al, al, 4096, 2048, 64, al, 4096, 2048, 64, 16,
+                                      al, null)
+
+    for call in [lambda: prompt(al, 1 << 23), lambda: prompt(null, 0, B=1 << 23),
+                 lambda: prompt(al, 1 << 20, ns=8, ws=al), lambda: prompt(al, 1 << 18, ns=17, ws=al),
+                 lambda: shared(1 << 23, 64), lambda: rope(1 << 27)]:
+        assert call() == 1 and "too many rows" in _err(lib)
+    assert prompt(al, 1, ns=2, ws=odd) == 1 and "aligned" in _err(lib)
+    assert shared(2, 5000, odd) == 1 and "aligned" in _err(lib)
+
+
 def test_workspace_sizes(lib):
     from laprune_amd import _native as N
     assert N.size_query("lap_prompt_attention_workspace_size", 10, 8, 128, 1) == 0
