@@ -598,7 +598,7 @@ int lap_qk_rope_append(const void* q, int64_t q_st, int64_t q_sh,
  *   K/V     [B][Hkv][Tk][D] strides (sb, sh, st, 1); no row past Tk is read
  *   tokens_per_tile, nsplit   of lap_prompt_shape; max_keys as given to it
  *   workspace   for nsplit > 1: lap_prompt_attention_workspace_size(tokens, ...), tokens =
- *           Tq (packed) or B * Tq.  Calls that share one must be ordered.
+ *           Tq (packed) or B * Tq, 16-byte aligned.  Calls that share one must be ordered.
  * D 64, 128 or 256, fp16/bf16, Hq / Hkv up to 128, every row 16-byte aligned. */
 int lap_prompt_attention_workspace_size(int64_t tokens, int Hq, int D, int nsplit, size_t* bytes);
 int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,

@@ -102,6 +102,7 @@ struct FlashArgs {
   int Tq, Tk;        // query tokens (of a sequence, or packed), cache rows
   const int4* tiles; // packed form
   int bt;            // tokens per tile
+  int n_tiles;
   int tps;           // uniform form: tiles per sequence
   int nsplit, per_split;
   float c;           // scale * log2(e)
@@ -127,7 +128,7 @@ struct FlashTile {
   int key0;            // token j sees keys [0, key0 + j + 1), or
   const int32_t* lens; // [0, min(hi, lens[8 j])) where not null
   int lo, hi;          // keys of this workgroup
-  int split;
+  int split, parts;    // this part of the keys, and how many hold any (1: no merge)
 };
 
 // Copies of key tiles straight into LDS, 16 bytes per lane: a wave writes 1 KB of
@@ -465,7 +466,7 @@ __device__ __forceinline__ void flash(const FlashArgs& a, const FlashTile& t,
 
   w.l += __shfl_xor(w.l, 32, 64);
   if (!live) return;
-  if (a.nsplit == 1) {
+  if (t.parts == 1) {
     // weights that sum to zero (no key, or all scores -inf) give zeros
     const float inv = w.l == 0.f ? 0.f : 1.0f / w.l;
     uint16_t* op = t.out + j * t.o_st + head * a.o_sh;
@@ -506,12 +507,24 @@ __device__ __forceinline__ bool prompt_tile(const FlashArgs& a, int ti, PromptTi
   p = {ti % a.B, i * a.bt, min(a.bt, a.Tq - i * a.bt), a.Tk - a.Tq + i * a.bt};
   return true;
 }
+// The keys of a tile's last token, and the parts that they fill (all but the last of
+// per_split keys); no key past the cache is read.
+__device__ __forceinline__ int prompt_keys(const FlashArgs& a, const PromptTile& p) {
+  return max(min(p.key0 + p.n, a.Tk), 0);
+}
+__device__ __forceinline__ int prompt_parts(const FlashArgs& a, int keys) {
+  return min(max((keys - 1) / a.per_split + 1, 1), a.nsplit);
+}
 __device__ __forceinline__ int64_t prompt_row(const FlashArgs& a, const PromptTile& p) {
   return (a.tiles ? 0 : (int64_t)p.b * a.Tq) + p.q0;
 }
 
-// Workgroup -> (tile, split, KV head), the KV head fastest: consecutive workgroups go
-// to different XCDs, so an XCD's L2 holds the keys of few heads.
+// Workgroup -> (split, tile, KV head), the KV head fastest: consecutive workgroups go
+// to different XCDs, so an XCD's L2 holds the keys of few heads.  Split by split: all
+// first parts, which are whole, start before the last ones, which causal tiles leave short
+// or empty (with a tile's splits side by side an even number of them put the same split on
+// the same XCDs: one prompt of 16384 tokens, 4 heads on 1, D = 128, two splits 405 us, 310
+// so).
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
 void prompt_kernel(FlashArgs a) {
@@ -519,11 +532,14 @@ void prompt_kernel(FlashArgs a) {
       s_v[2 * bn<D>() * D * 2];
   const int hkv = blockIdx.x % a.Hkv;
   const int rest = blockIdx.x / a.Hkv;
-  const int split = rest % a.nsplit;
+  const int split = rest / a.n_tiles, tile = rest % a.n_tiles;
   PromptTile p;
-  if (!prompt_tile(a, rest / a.nsplit, p)) return;
-  const int64_t qb = a.tiles ? 0 : p.b;
+  if (!prompt_tile(a, tile, p)) return;
+  const int keys = prompt_keys(a, p);
   FlashTile t;
+  t.parts = prompt_parts(a, keys);
+  if (split >= t.parts) return;
+  const int64_t qb = a.tiles ? 0 : p.b;
   t.n = p.n;
   t.key0 = p.key0;
   t.lens = nullptr;
@@ -534,11 +550,9 @@ void prompt_kernel(FlashArgs a) {
   t.o_st = a.o_st;
   t.k = a.k + (int64_t)p.b * a.k_sb + (int64_t)hkv * a.k_sh;
   t.v = a.v + (int64_t)p.b * a.v_sb + (int64_t)hkv * a.v_sh;
-  // the last split takes what is left; no key past the cache is read
-  const int keys = min(p.key0 + p.n, a.Tk);
   t.split = split;
-  t.lo = (int)min((int64_t)split * a.per_split, (int64_t)keys);
-  t.hi = split == a.nsplit - 1 ? keys : min(keys, t.lo + a.per_split);
+  t.lo = split * a.per_split;
+  t.hi = split == t.parts - 1 ? keys : t.lo + a.per_split;
   flash<DT, D, false>(a, t, s_k, s_v);
 }
 
@@ -554,6 +568,7 @@ void shared_kernel(FlashArgs a) {
   const int hkv = blockIdx.x % a.Hkv;
   const int it = blockIdx.x / a.Hkv, n_pre = a.psplit * a.pblocks;
   FlashTile t;
+  t.parts = a.nsplit;
   int b, kb = 0;
   if (it < n_pre) {
     b = it / a.psplit * a.bt;
@@ -598,7 +613,7 @@ template <> struct Vals<128> { typedef float2 type; };
 template <> struct Vals<256> { typedef float4 type; };
 
 template <int DT, int D, int WPR>
-__device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, bool live,
+__device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, int parts, bool live,
                                           uint16_t* out) {
   constexpr int V = D / 64;
   typedef typename Vals<D>::type vals;
@@ -608,8 +623,8 @@ __device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, bool 
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.nsplit;
     const vals* po = reinterpret_cast<const vals*>(a.part_o + row * a.nsplit * D) + lane;
     // 64 splits at a time: lane s holds split s's weight
-    for (int s0 = 0; s0 < a.nsplit; s0 += 64) {
-      const int n = min(64, a.nsplit - s0);
+    for (int s0 = 0; s0 < parts; s0 += 64) {
+      const int n = min(64, parts - s0);
       const float2 x = lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
       vals v[kMergeAhead];
       const auto request = [&](int s) {
@@ -664,21 +679,24 @@ __device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, bool 
   for (int e = 0; e < V; ++e) out[lane * V + e] = st16<DT>(o[e] * inv);
 }
 
-// A row per (tile, token, head); only rows of a tile are written.
+// A row per (tile, token, head); only rows of a tile with more than one part are written.
 template <int DT, int D, int WPR>
 __global__ __launch_bounds__(kMergeThreads) void prompt_merge_kernel(FlashArgs a, int rows) {
   const int r = blockIdx.x * (4 / WPR) + (threadIdx.x >> 6) / WPR;
   const int h = r % a.Hq, rest = r / a.Hq, j = rest % a.bt;
   PromptTile p{};
-  const bool live = r < rows && prompt_tile(a, rest / a.bt, p) && j < p.n;
+  int parts = 1;
+  if (r < rows && prompt_tile(a, rest / a.bt, p) && j < p.n)
+    parts = prompt_parts(a, prompt_keys(a, p));
+  const bool live = parts > 1;
   uint16_t* out = a.out + (a.tiles ? 0 : p.b) * a.o_sb + (int64_t)(p.q0 + j) * a.o_st + h * a.o_sh;
-  merge_row<DT, D, WPR>(a, (prompt_row(a, p) + j) * a.Hq + h, live, out);
+  merge_row<DT, D, WPR>(a, (prompt_row(a, p) + j) * a.Hq + h, parts, live, out);
 }
 
 template <int DT, int D, int WPR>
 __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(FlashArgs a, int rows) {
   const int r = blockIdx.x * (4 / WPR) + (threadIdx.x >> 6) / WPR;
-  merge_row<DT, D, WPR>(a, r, r < rows, a.out + (int64_t)r * D);
+  merge_row<DT, D, WPR>(a, r, a.nsplit, r < rows, a.out + (int64_t)r * D);
 }
 
 int merge_waves(int nsplit) { return nsplit > kMergeFew ? 4 : 1; }
@@ -733,6 +751,42 @@ int check_heads(const char* fn, int Hq, int Hkv, int D) {
   return LAP_OK;
 }
 
+// Parts of the keys for `items` (tile, KV head) pairs with up to max_keys keys each, `fresh`
+// of them new tokens'.  Estimated time in tiles of 64 keys of a workgroup that has its CU
+// to itself (1.2 us at D = 128).  Two share a CU below D = 256: the second one slows both
+// down, to 1.65 when all CUs are full, less while few are or parts end early.  A merge
+// costs its launch and the partial sums.  Fitted to 53 shapes of 1 to 16 sequences, at most
+// 1024 items and 256 to 65536 keys: 1.2 % behind the best count on average, where filling
+// one round of workgroups with parts of at least 512 keys was 10 % (16384 tokens of 2 heads
+// on 2, 3 parts 179 us, 1 301, 4 211; 1200 tokens behind 64336, 32 heads on 8, 6 parts 1280,
+// 1 1646; 2048 tokens of 8 heads on 4, D = 256, 3 parts 55, 4 76, 1 100; 2048 tokens of 32
+// heads on 8, 1 part 51, 2 76).
+int prompt_splits(int64_t items, double fresh, int max_keys, int D) {
+  if (items == 0 || max_keys == 0) return 1;
+  const int64_t slots = D == 256 ? 256 : 512;  // workgroups that run at a time
+  const double seen = 1 - std::min(fresh, (double)max_keys) / (2.0 * max_keys);  // on average
+  const double work = items * seen * max_keys / 64;
+  double least = 0;
+  int best = 1;
+  for (int64_t n = 1; n == 1 || (n <= 32 && n * kGran <= max_keys && items * n <= 2048); ++n) {
+    const int64_t per = ((max_keys + n - 1) / n + kGran - 1) / kGran,
+                  ns = (max_keys + per * kGran - 1) / (per * kGran);
+    const double parts = ns * seen + 1 - seen, live = items * parts;  // that hold keys
+    const double fill = std::min(1.0, work / (live * per));
+    double cost = per;
+    if (live > slots)
+      cost = D == 256 ? work / slots + per * fill : 1.65 * work / slots + per * fill * fill / 2;
+    else if (live > 256)
+      cost = per * (1.1 + (0.1 + 0.45 * (live - 256) / 256) * (2 * fill - 1));
+    cost += 6 + (ns > 1 ? 4 + items * (2 + parts) / 80 : 0);
+    if (n == 1 || cost < 0.98 * least) {
+      least = cost;
+      best = (int)ns;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 }  // namespace lap
 
@@ -746,18 +800,10 @@ extern "C" int lap_prompt_shape(int total, int B, int tiles, int max_keys, int H
   int s = check_heads("lap_prompt_shape", Hq, Hkv, D);
   if (s != LAP_OK) return s;
   const int bt = kRows / (Hq / Hkv), bound = total / bt + std::min(B, total);
-  // 512 workgroups run at a time (two to a CU).  Fewer than 256 of them share out the
-  // keys, at least 512 each: a part below costs more in the merge than it gives, and a
-  // 513th workgroup starts when the others are done (300 tokens behind 36057, 68
-  // workgroups: 6 parts 198 us, 8 parts 265; 512 tokens, 136 workgroups: 1 part 17.8, 2
-  // parts of 256 39.6).
   const int64_t items = (int64_t)(tiles > 0 ? std::min(tiles, bound) : bound) * Hkv;
-  int ns = 1;
-  if (items > 0 && items < 256)
-    ns = (int)std::max<int64_t>(1, std::min<int64_t>({512 / items, max_keys / 512, 32}));
   *tokens_per_tile = bt;
   *n_tiles = bound;
-  *nsplit = ns;
+  *nsplit = prompt_splits(items, (double)total / B, max_keys, D);
   return LAP_OK;
 }
 
@@ -812,6 +858,7 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
   a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = G; a.Tq = Tq; a.Tk = Tk;
   a.tiles = reinterpret_cast<const int4*>(tiles);
   a.bt = tokens_per_tile;
+  a.n_tiles = (int)all_tiles;
   a.tps = tps;
   a.nsplit = nsplit;
   a.per_split =
