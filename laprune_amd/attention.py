@@ -112,8 +112,8 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     if plan.total != q.shape[0] or plan.B != k.shape[0]:
         raise RuntimeError(f"prompt_attention: a plan of {plan.total} tokens of {plan.B} sequences, "
                            f"got {q.shape[0]} of {k.shape[0]}")
-    if plan.lens is not None and plan.max_keys > k.shape[2] and plan.total:
-        raise RuntimeError(f"prompt_attention: {plan.max_keys} keys exceed the {k.shape[2]} rows "
+    if plan.lens is not None and plan.longest > k.shape[2] and plan.total:
+        raise RuntimeError(f"prompt_attention: {plan.longest} keys exceed the {k.shape[2]} rows "
                            "of the caches")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)

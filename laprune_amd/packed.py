@@ -38,6 +38,7 @@ class PackedPrompts:
     tiles  int32 [n, 4]   the attention's blocks of queries, for the heads given to
                           ``pack_prompts`` (None without them)
     lens, cached: the lengths as host lists, or None when they were device tensors
+    longest: the most keys of a sequence, when the lengths are known (else max_keys)
     """
 
     def __init__(self, batch, total, max_keys, heads, shape, starts, seq, pos, tiles, lens, cached):
@@ -45,6 +46,7 @@ class PackedPrompts:
         self.heads, self.shape = heads, shape
         self.starts, self.seq, self.pos, self.tiles = starts, seq, pos, tiles
         self.lens, self.cached = lens, cached
+        self.longest = max_keys if lens is None else max(map(int.__add__, lens, cached))
 
 
 def _host(v, name: str, batch: int | None = None) -> list[int]:

@@ -513,3 +513,21 @@ def test_batches_past_one_launch_keep_the_library(dev, Hq, Hkv, Tq):
     for B, fits in [(most, True), (most + 1, False)]:
         x, y = (t.expand(B, -1, -1, -1) for t in (q, k))
         assert _prompt_kernel_fits(x, y, y) == fits
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_a_loose_bound_of_the_keys(dev, D):
+    """max_keys may pass the caches, with lengths of either kind; only real keys are checked."""
+    from laprune_amd.attention import prompt_attention
+    from laprune_amd.packed import pack_prompts
+    lens, cached = [40, 0, 7], [30, 9, 3]
+    q, k, v = _attn_case(dev, torch.bfloat16, 4, 2, D, lens, cached)
+    heads = dict(num_q_heads=4, num_kv_heads=2, head_dim=D)
+    for most in (70, 4096, 1 << 29):
+        for plan in (pack_prompts(lens, cached, max_keys=most, device=dev, **heads),
+                     pack_prompts(*(torch.tensor(x, dtype=torch.int32, device=dev) for x in (lens, cached)),
+                                  total=47, max_keys=most, **heads)):
+            _check_prompt(prompt_attention(q, k, v, plan), q, k, v, lens, cached)
+    with pytest.raises(RuntimeError, match="70 keys exceed the 69 rows"):
+        prompt_attention(q, k[:, :, :69], v[:, :, :69],
+                         pack_prompts(lens, cached, max_keys=4096, device=dev, **heads))
