@@ -523,7 +523,7 @@ __device__ __forceinline__ int64_t prompt_row(const FlashArgs& a, const PromptTi
 // to different XCDs, so an XCD's L2 holds the keys of few heads.  Split by split: all
 // first parts, which are whole, start before the last ones, which causal tiles leave short
 // or empty (with a tile's splits side by side an even number of them put the same split on
-// the same XCDs: one prompt of 16384 tokens, 4 heads on 1, D = 128, two splits 405 us, 310
+// the same XCDs: one prompt of 16384 tokens, 4 heads on 1, D = 128, two splits 405 us, 312
 // so).
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
@@ -600,42 +600,50 @@ void shared_kernel(FlashArgs a) {
 }
 
 // out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) of one row by WPR waves: a wave takes
-// every WPR-th batch of kMergeAhead splits, its lanes D / 64 of the row's values each, and
-// the first wave adds the waves up.  Four waves where there are more than kMergeFew splits
-// (their batches come one after the other), one where there are few (a decode step of 8
-// sequences behind 30000 tokens, 8 heads on 1: 33.2 us with one wave, 20.0 with four; a
-// prompt of 300 tokens behind 36057, 7 splits: 192.7 and 200.0).
+// every WPR-th batch of kMergeAhead splits, and the first wave adds the waves up.  Four
+// waves where there are more than kMergeFew splits (their batches come one after the
+// other), one where there are few (a decode step of 8 sequences behind 30000 tokens, 8
+// heads on 1: 33.2 us with one wave, 20.0 with four; a prompt of 300 tokens behind 36057, 7
+// splits: 192.7 and 200.0); a wave of its own then has 16 bytes of each split to a lane
+// and up to four rows (38912 rows of 6 splits, D = 128: 31.6 us with one row, 22.6 with
+// two, 5.3 TB/s; 16384 of 4 splits 12.9 and 9.2).
 constexpr int kMergeAhead = 8, kMergeFew = 16, kMergeThreads = 256;
-template <int D>
+// Lanes of a row: four values each where a wave has rows of its own.
+template <int D, int WPR>
+constexpr int merge_lanes() {
+  return WPR == 1 ? D / 4 : 64;
+}
+template <int V>
 struct Vals;
-template <> struct Vals<64> { typedef float type; };
-template <> struct Vals<128> { typedef float2 type; };
-template <> struct Vals<256> { typedef float4 type; };
+template <> struct Vals<1> { typedef float type; };
+template <> struct Vals<2> { typedef float2 type; };
+template <> struct Vals<4> { typedef float4 type; };
 
 template <int DT, int D, int WPR>
 __device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, int parts, bool live,
                                           uint16_t* out) {
-  constexpr int V = D / 64;
-  typedef typename Vals<D>::type vals;
-  const int lane = threadIdx.x & 63, part = (threadIdx.x >> 6) % WPR;
+  constexpr int LPR = merge_lanes<D, WPR>(), V = D / LPR;
+  typedef typename Vals<V>::type vals;
+  const int lane = threadIdx.x % LPR, lane0 = (threadIdx.x & 63) - lane;
+  const int part = (threadIdx.x >> 6) % WPR;
   float M = -INFINITY, l = 0.f, o[V] = {};
   if (live) {
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.nsplit;
     const vals* po = reinterpret_cast<const vals*>(a.part_o + row * a.nsplit * D) + lane;
-    // 64 splits at a time: lane s holds split s's weight
-    for (int s0 = 0; s0 < parts; s0 += 64) {
-      const int n = min(64, parts - s0);
+    // LPR splits at a time: the row's lane s holds split s's weight
+    for (int s0 = 0; s0 < parts; s0 += LPR) {
+      const int n = min(LPR, parts - s0);
       const float2 x = lane < n ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
       vals v[kMergeAhead];
       const auto request = [&](int s) {
 #pragma unroll
-        for (int i = 0; i < kMergeAhead; ++i) v[i] = po[(int64_t)(s0 + min(s + i, n - 1)) * 64];
+        for (int i = 0; i < kMergeAhead; ++i) v[i] = po[(int64_t)(s0 + min(s + i, n - 1)) * LPR];
       };
       int s = part * kMergeAhead;
       if (s < n) request(s);
       float top = x.x;
 #pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+      for (int d = LPR / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
       top = fmaxf(top, M);
       const float base = top == -INFINITY ? 0.f : top;
       // a split without keys of this row: weight 0, and its values are 0
@@ -643,7 +651,7 @@ __device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, int p
       const float before = __builtin_amdgcn_exp2f(M - base);
       float sum = x.y * w;
 #pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+      for (int d = LPR / 2; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
       l = l * before + sum;
 #pragma unroll
       for (int e = 0; e < V; ++e) o[e] *= before;
@@ -651,7 +659,7 @@ __device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, int p
       while (s < n) {
 #pragma unroll
         for (int i = 0; i < kMergeAhead; ++i) {
-          const float ws = s + i < n ? __shfl(w, s + i, 64) : 0.f;
+          const float ws = s + i < n ? __shfl(w, lane0 + s + i, 64) : 0.f;
           const float* f = reinterpret_cast<const float*>(&v[i]);
 #pragma unroll
           for (int e = 0; e < V; ++e) o[e] = ws == 0.f ? o[e] : __builtin_fmaf(f[e], ws, o[e]);
@@ -675,14 +683,25 @@ __device__ __forceinline__ void merge_row(const FlashArgs& a, int64_t row, int p
   }
   if (!live) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
+  if constexpr (V == 4) {
+    const uint2 x = make_uint2(pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv));
+    *reinterpret_cast<uint2*>(out + lane * 4) = x;
+  } else {
 #pragma unroll
-  for (int e = 0; e < V; ++e) out[lane * V + e] = st16<DT>(o[e] * inv);
+    for (int e = 0; e < V; ++e) out[lane * V + e] = st16<DT>(o[e] * inv);
+  }
+}
+
+template <int D, int WPR>
+__device__ __forceinline__ int merge_row_of() {
+  constexpr int threads = merge_lanes<D, WPR>() * WPR;  // of a row
+  return blockIdx.x * (kMergeThreads / threads) + threadIdx.x / threads;
 }
 
 // A row per (tile, token, head); only rows of a tile with more than one part are written.
 template <int DT, int D, int WPR>
 __global__ __launch_bounds__(kMergeThreads) void prompt_merge_kernel(FlashArgs a, int rows) {
-  const int r = blockIdx.x * (4 / WPR) + (threadIdx.x >> 6) / WPR;
+  const int r = merge_row_of<D, WPR>();
   const int h = r % a.Hq, rest = r / a.Hq, j = rest % a.bt;
   PromptTile p{};
   int parts = 1;
@@ -695,16 +714,19 @@ __global__ __launch_bounds__(kMergeThreads) void prompt_merge_kernel(FlashArgs a
 
 template <int DT, int D, int WPR>
 __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(FlashArgs a, int rows) {
-  const int r = blockIdx.x * (4 / WPR) + (threadIdx.x >> 6) / WPR;
+  const int r = merge_row_of<D, WPR>();
   merge_row<DT, D, WPR>(a, r, a.nsplit, r < rows, a.out + (int64_t)r * D);
 }
 
 int merge_waves(int nsplit) { return nsplit > kMergeFew ? 4 : 1; }
-int64_t merge_blocks(int64_t rows, int nsplit) { return (rows * merge_waves(nsplit) + 3) / 4; }
+int64_t merge_blocks(int64_t rows, int nsplit, int D) {
+  const int per = merge_waves(nsplit) > 1 ? 1 : kMergeThreads / (D / 4);
+  return (rows + per - 1) / per;
+}
 
 template <bool SHARED, int DT, int D, int WPR>
 void launch_merge(const FlashArgs& a, int64_t rows, hipStream_t st) {
-  const dim3 g((unsigned)merge_blocks(rows, a.nsplit)), threads(kMergeThreads);
+  const dim3 g((unsigned)merge_blocks(rows, a.nsplit, D)), threads(kMergeThreads);
   if constexpr (SHARED)
     hipLaunchKernelGGL((shared_merge_kernel<DT, D, WPR>), g, threads, 0, st, a, (int)rows);
   else hipLaunchKernelGGL((prompt_merge_kernel<DT, D, WPR>), g, threads, 0, st, a, (int)rows);
@@ -756,11 +778,11 @@ int check_heads(const char* fn, int Hq, int Hkv, int D) {
 // to itself (1.2 us at D = 128).  Two share a CU below D = 256: the second one slows both
 // down, to 1.65 when all CUs are full, less while few are or parts end early.  A merge
 // costs its launch and the partial sums.  Fitted to 53 shapes of 1 to 16 sequences, at most
-// 1024 items and 256 to 65536 keys: 1.2 % behind the best count on average, where filling
+// 1024 items and 256 to 65536 keys: 1.7 % behind the best count on average, where filling
 // one round of workgroups with parts of at least 512 keys was 10 % (16384 tokens of 2 heads
-// on 2, 3 parts 179 us, 1 301, 4 211; 1200 tokens behind 64336, 32 heads on 8, 6 parts 1280,
-// 1 1646; 2048 tokens of 8 heads on 4, D = 256, 3 parts 55, 4 76, 1 100; 2048 tokens of 32
-// heads on 8, 1 part 51, 2 76).
+// on 2, 3 parts 172 us, 1 301, 4 202; 1200 tokens behind 64336, 32 heads on 8, 6 parts 1278,
+// 1 1651; 2048 tokens of 8 heads on 4, D = 256, 3 parts 54, 4 75, 1 100; 2048 tokens of 32
+// heads on 8, 1 part 52, 2 66).
 int prompt_splits(int64_t items, double fresh, int max_keys, int D) {
   if (items == 0 || max_keys == 0) return 1;
   const int64_t slots = D == 256 ? 256 : 512;  // workgroups that run at a time
@@ -872,7 +894,7 @@ extern "C" int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, i
   LAP_CHECK(grid <= kMaxBlocks256, "lap_prompt_attention: too many rows");
   const int64_t tile_rows = all_tiles * tokens_per_tile * Hq;  // at most 128 * grid
   if (nsplit > 1) {
-    LAP_CHECK(merge_blocks(tile_rows, nsplit) <= kMaxBlocks256,
+    LAP_CHECK(merge_blocks(tile_rows, nsplit, D) <= kMaxBlocks256,
               "lap_prompt_attention: too many rows");
     LAP_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
               "lap_prompt_attention: workspace must be 16-byte aligned");
@@ -979,7 +1001,7 @@ extern "C" int lap_shared_attn_decode(const void* q, int64_t q_sb, int64_t q_sh,
   const int64_t rows = (int64_t)B * Hq;
   const int64_t grid =
       ((int64_t)sh.pblocks * sh.psplit + (int64_t)B * (sh.nsplit - sh.psplit)) * Hkv;
-  LAP_CHECK(grid <= kMaxBlocks256 && merge_blocks(rows, sh.nsplit) <= kMaxBlocks256,
+  LAP_CHECK(grid <= kMaxBlocks256 && merge_blocks(rows, sh.nsplit, D) <= kMaxBlocks256,
             "lap_shared_attn_decode: too many rows");
   if (sh.nsplit > 1) {
     LAP_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
