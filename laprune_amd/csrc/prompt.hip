@@ -178,6 +178,16 @@ struct Rows {
   float m, l;         // maximum (log2, scaled; equal in the lane pair) and this lane's sum
 };
 
+// Where a wave has 512 registers (D = 256), products accumulate in the upper 256, which
+// vector instructions do not reach.  o^T stays there: after the few places that do compute
+// with it, it goes back, instead of all of it moving to and fro with every tile.
+template <int DT, int D>
+__device__ __forceinline__ void in_acc(Rows<DT, D>& w) {
+  if constexpr (D == 256)
+#pragma unroll
+    for (int dc = 0; dc < D / 32; ++dc) asm volatile("" : "+a"(w.o[dc]));
+}
+
 // A row's maximum is raised only when a tile exceeds it by more than this, so weights
 // go up to 2^8 before the division by their sum: no rounding differs for it, and the
 // o^T registers are rescaled in few tiles.
@@ -270,8 +280,10 @@ __device__ __forceinline__ void weights(Rows<DT, D>& w, Scores<D>& s, Weights<D>
     const float alpha = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - m_new);
     w.m = m_new;
     w.l *= alpha;
+    in_acc<DT, D>(w);
 #pragma unroll
     for (int dc = 0; dc < DC; ++dc) w.o[dc] *= alpha;
+    in_acc<DT, D>(w);
   }
   const float base = w.m == -INFINITY ? 0.f : w.m;
   float sum[2] = {0.f, 0.f};
@@ -344,6 +356,7 @@ __device__ __forceinline__ void values_masked(Rows<DT, D>& w, const LaneAddr<D>&
     values<DT, D>(w, la, vb, pk);
     return;
   }
+  in_acc<DT, D>(w);
 #pragma unroll 1
   for (int r = 0; r < kBN && kt + r < hi; ++r) {
     // the weight of key r: register 4 * (r / 8) + r % 4 of half r / 32, in the lane of
@@ -365,6 +378,7 @@ __device__ __forceinline__ void values_masked(Rows<DT, D>& w, const LaneAddr<D>&
         w.o[dc][i] = sees ? __builtin_fmaf(p, x, w.o[dc][i]) : w.o[dc][i];
       }
   }
+  in_acc<DT, D>(w);
 }
 
 template <int DT, int D, bool SHARED>
@@ -419,6 +433,7 @@ __device__ __forceinline__ void flash(const FlashArgs& a, const FlashTile& t,
   for (int dc = 0; dc < DC; ++dc)
 #pragma unroll
     for (int i = 0; i < 16; ++i) w.o[dc][i] = 0.f;
+  in_acc<DT, D>(w);
   w.m = -INFINITY;
   w.l = 0.f;
 
