@@ -801,7 +801,7 @@ int check_heads(const char* fn, int Hq, int Hkv, int D) {
 // 1024 items and 256 to 65536 keys: 1.7 % behind the best count on average, where filling
 // one round of workgroups with parts of at least 512 keys was 10 % (16384 tokens of 2 heads
 // on 2, 3 parts 172 us, 1 301, 4 202; 1200 tokens behind 64336, 32 heads on 8, 6 parts 1278,
-// 1 1651; 2048 tokens of 8 heads on 4, D = 256, 3 parts 54, 4 75, 1 100; 2048 tokens of 32
+// 1 1651; 2048 tokens of 8 heads on 4, D = 256, 3 parts 48, 4 66, 1 80; 2048 tokens of 32
 // heads on 8, 1 part 52, 2 66).
 int prompt_splits(int64_t items, double fresh, int max_keys, int D) {
   if (items == 0 || max_keys == 0) return 1;
