@@ -278,7 +278,9 @@ __device__ __forceinline__ void weights(Rows<DT, D>& w, Scores<D>& s, Weights<D>
   {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
                                                     __builtin_bit_cast(uint32_t, mx), false, false);
-    mx = fmaxf(__builtin_bit_cast(float, r[0]), __builtin_bit_cast(float, r[1])) * c;
+    // (a bit cast of a vector's element itself reads the vector's first one)
+    const uint32_t lower = r[0], upper = r[1];
+    mx = fmaxf(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper)) * c;
   }
   if (__ballot(mx > w.m + kSlack)) {  // also where m is -inf and a score is not
     const float m_new = mx > w.m + kSlack ? mx : w.m;
