@@ -6,7 +6,8 @@
 // Both are, per KV head, a block of rows (a row is one query head of one token) over
 // a range of keys:
 //   o[r] = sum_{t < lim[r]} 2^(c (q[r].k[t]) - m[r]) v[t] / sum of the same weights,
-// c = scale * log2(e), m the row's running maximum (one pass over the keys, fp32).
+// c = scale * log2(e), m close to the row's running maximum (one pass over the keys, fp32;
+// kSlack and kUp say how close).
 //
 // Products are 32x32x16 MFMAs with the scores transposed, S^T = K Q^T: a lane then
 // holds 16 keys of one query (column lane % 32, keys 8 i + 4 (lane / 32) + e), so a
@@ -71,7 +72,8 @@ __device__ __forceinline__ f32x16 mfma32(i16x8 a, i16x8 b, f32x16 c) {
 }
 
 // Two weights in the data type, round to nearest even.  The weights enter the second
-// product in 16 bits (half a step, 2^-9 or 2^-12 of each); their sum stays fp32.
+// product in 16 bits (off by up to half a step, 2^-8 or 2^-11 of each; fp16 below its
+// normal range, see kUp); their sum stays fp32.
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (DT == LAP_DTYPE_F16) {
@@ -179,7 +181,7 @@ template <int DT, int D>
 struct Rows {
   i16x8 qf[D / 16];   // Q^T operand
   f32x16 o[D / 32];   // o^T: rows d = 32 dc + (i & 3) + 8 (i >> 2) + 4 (lane / 32)
-  float m, l;         // maximum (log2, scaled; equal in the lane pair) and this lane's sum
+  float m, l;         // exponent of the weights (log2; equal in the lane pair), this lane's sum
 };
 
 // Where a wave has 512 registers (D = 256), products accumulate in the upper 256, which
@@ -197,6 +199,13 @@ __device__ __forceinline__ void in_acc(Rows<DT, D>& w) {
 // go up to 2^8 before the division by their sum: no rounding differs for it, and the
 // o^T registers are rescaled in few tiles.
 constexpr float kSlack = 8.f;
+// The exponent m that a row's weights are relative to lies this far below its maximum.  fp16
+// has no relative steps below 2^-14 and nothing below 2^-25: with weights of up to 2^15 (and the
+// slack in it) those of 2^-21 and more of the largest keep half a step, and what lies below
+// 2^-32 of it is lost, where 65000 keys of 2^-25 each would still be 0.2 % of the row (same time:
+// one prompt of 16384 tokens 2130 and 2142 us in fp16).  The sum and o^T carry the factor too.
+template <int DT>
+constexpr float kUp = DT == LAP_DTYPE_F16 ? 7.f : 0.f;
 
 // LDS addresses of a lane's operands in the first buffer.  The others are a constant
 // away, or, within a row, a constant XORed to the chunk's bits: rows of 128 bytes or
@@ -282,8 +291,9 @@ __device__ __forceinline__ void weights(Rows<DT, D>& w, Scores<D>& s, Weights<D>
     const uint32_t lower = r[0], upper = r[1];
     mx = fmaxf(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper)) * c;
   }
-  if (__ballot(mx > w.m + kSlack)) {  // also where m is -inf and a score is not
-    const float m_new = mx > w.m + kSlack ? mx : w.m;
+  const float top = mx - kUp<DT>;
+  if (__ballot(top > w.m + kSlack)) {  // also where m is -inf and a score is not
+    const float m_new = top > w.m + kSlack ? top : w.m;
     const float alpha = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - m_new);
     w.m = m_new;
     w.l *= alpha;

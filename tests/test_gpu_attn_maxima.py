@@ -87,3 +87,37 @@ def test_every_key_as_the_largest_of_a_shared_prefix(dev, dtype, D):
     for i in range(B):
         for h in (0, 3):
             check(got[i, h], *attend64(q[i, h], k[i, 0], v[i, 0], all_keys, 1 / math.sqrt(D), dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("at", [0, 5, 40000])
+@pytest.mark.parametrize("nsplit", [1, 5])
+def test_many_small_weights_beside_a_large_one(dev, dtype, D, at, nsplit):
+    """Key `at` weighs 1 and its value is 0; 65000 others weigh 2^-18 to 2^-30 each and their
+    values are 1, so the output is the others' share.  A weight is off by half a step of its
+    own in the normal range, and in fp16 below that by half a step of 2^-24 at weights that
+    are at least 2^7 where the row's largest is 1 (half a step of 2^-31)."""
+    from laprune_amd.attention import prompt_attention
+    from laprune_amd.packed import pack_prompts
+    T, n = 65001, 5
+    k = torch.zeros(1, 1, T, D, dtype=dtype, device=dev)
+    k[..., at, 0] = 8.0
+    v = torch.ones(1, 1, T, D, dtype=dtype, device=dev)
+    v[..., at, :] = 0.0
+    power = torch.tensor([18.0, 23.0, 25.2, 27.0, 30.0], device=dev)
+    q = torch.zeros(n, 1, D, dtype=dtype, device=dev)
+    q[:, 0, 0] = (power * math.log(2) * math.sqrt(D) / 8).to(dtype)
+    plan = pack_prompts([n], [T - n], device=dev, num_q_heads=1, num_kv_heads=1, head_dim=D)
+    plan.shape = (*plan.shape[:2], nsplit)
+    got = prompt_attention(q, k, v, plan)[:, 0].double()
+    seen = torch.arange(T - n + 1, T + 1, device=dev).double()[:, None] - 1
+    w = (-8 * q[:, :, 0].double() / math.sqrt(D)).exp()
+    want = (seen * w / (1 + seen * w)).expand(n, D)
+    # fp32 (half steps): the score and the exponential's argument up to 30, each twice, and the
+    # sums of 16 weights in a lane per tile, of its tiles and of the parts
+    tol = want * (torch.finfo(dtype).eps + 2.0 ** -24 * (8 + 4 * 30 + 2 * (16 + 2 * (T // 64 + 1) + 8)))
+    if dtype == torch.float16:
+        tol = tol + seen * 2.0 ** -32 + 2.0 ** -25  # the weights' and the output's smallest steps
+    d = (got - want).abs()
+    assert bool((d <= tol).all()), (d / tol)[:, 0].tolist()
