@@ -511,8 +511,7 @@ class LAPruneLlama:
         self._check_room(T)
         if T > 1 and self._packs():
             return self._prefill(list(range(self.B)), list(input_ids))
-        pos = torch.arange(T, device=self.dev)[None].expand(self.B, T)
-        self._pos = pos
+        pos = self._pos = torch.arange(T, device=self.dev).repeat(self.B, 1)  # the kernels' layout
         return self._forward(input_ids.to(self.dev), pos)
 
     @torch.no_grad()
