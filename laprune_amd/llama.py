@@ -27,6 +27,7 @@ downloads anything (build it from a local ``LlamaConfig``).
 from __future__ import annotations
 
 import functools
+import inspect
 import math
 from dataclasses import dataclass, field
 from types import MethodType
@@ -213,6 +214,18 @@ def _step_mask(model, batch: int, device):
     return torch.ones((batch, 1, 1, 1), dtype=torch.bool, device=device)
 
 
+def _hands_masks_through(model) -> bool:
+    """Whether a 4-D mask reaches the attention layers as it is: the model's code builds
+    its masks with transformers' function."""
+    f = inspect.unwrap(type(model.model).forward)
+    try:
+        from transformers.masking_utils import create_causal_mask
+    except ImportError:
+        return False
+    return ("forward" not in model.model.__dict__ and
+            getattr(f, "__globals__", {}).get("create_causal_mask") is create_causal_mask)
+
+
 @dataclass
 class LAPruneSettings:
     """Decode settings (the reference's ``draft_kwargs`` keys on this path)."""
@@ -284,6 +297,11 @@ class LAPruneLlama:
             attn.forward = self._make_forward(i, attn)
         _fuse_decode_ops(model)
         self._mask = _step_mask(model, batch, self.dev)
+        # the mask of a packed pass: every layer's attention ignores it, and without one the
+        # model's code takes positions that start anew for sequences and builds a mask of the
+        # whole pass squared
+        self._packed_mask = (torch.ones((1, 1, 1, 1), dtype=torch.bool, device=self.dev)
+                             if _hands_masks_through(model) else None)
         self._plan = None    # tables of the packed prompts being prefilled
         self._row = None     # sequence being prefilled alone without them
         self._pos = None     # positions of the eager step being run
@@ -466,11 +484,8 @@ class LAPruneLlama:
                                "model was wrapped with (wrap it with a larger capacity)")
 
     def _forward(self, ids: torch.Tensor, pos: torch.Tensor, keep=1) -> torch.Tensor:
-        # every layer's attention ignores the mask (a packed pass would have one of its
-        # whole length squared built from the positions)
-        mask = self._mask
-        if mask is not None:
-            mask = mask[:ids.shape[0]] if ids.shape[1] == 1 or self._plan is not None else None
+        mask = (self._packed_mask if self._plan is not None else
+                self._mask if ids.shape[1] == 1 else None)
         out = self.model(input_ids=ids, attention_mask=mask, position_ids=pos, use_cache=False,
                          logits_to_keep=keep)
         return out.logits[:, -1] if isinstance(keep, int) else out.logits[0]
@@ -480,12 +495,15 @@ class LAPruneLlama:
         return self.D in (64, 128, 256) and self.Hq // self.Hkv <= 128
 
     def _prefill(self, rows: list[int], prompts: list[torch.Tensor]) -> torch.Tensor:
-        """One packed pass: prompts[i] behind what sequence rows[i] has cached; its last
-        position's logits [len(rows), V]."""
+        """Prompts[i] behind what sequence rows[i] has cached; their last positions' logits
+        [len(rows), V].  One packed pass, or one each for a model class whose masks are
+        built from the positions."""
         new = [int(p.numel()) for p in prompts]
         if not new or min(new) < 1:
             raise RuntimeError("a prompt needs at least one token")
         self._check_room(new, rows)
+        if len(rows) > 1 and self._packed_mask is None:
+            return torch.cat([self._prefill([b], [p]) for b, p in zip(rows, prompts)])
         lens = [0] * self.B
         for b, n in zip(rows, new):
             lens[b] = n
@@ -509,7 +527,7 @@ class LAPruneLlama:
         if any(n != 0 for n in self.lengths):
             raise RuntimeError("batched prefill needs empty caches (use reset())")
         self._check_room(T)
-        if T > 1 and self._packs():
+        if T > 1 and self._packs() and (self.B == 1 or self._packed_mask is not None):
             return self._prefill(list(range(self.B)), list(input_ids))
         pos = self._pos = torch.arange(T, device=self.dev).repeat(self.B, 1)  # the kernels' layout
         return self._forward(input_ids.to(self.dev), pos)
