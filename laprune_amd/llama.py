@@ -226,6 +226,13 @@ def _hands_masks_through(model) -> bool:
             getattr(f, "__globals__", {}).get("create_causal_mask") is create_causal_mask)
 
 
+def _rope_by_length(model) -> bool:
+    """Whether the model's rotary frequencies depend on the largest position of a pass."""
+    kinds = getattr(getattr(model.model, "rotary_emb", None), "rope_type", "default")
+    kinds = kinds.values() if isinstance(kinds, dict) else [kinds]
+    return any("dynamic" in k or k == "longrope" for k in kinds)
+
+
 @dataclass
 class LAPruneSettings:
     """Decode settings (the reference's ``draft_kwargs`` keys on this path)."""
@@ -497,12 +504,14 @@ class LAPruneLlama:
     def _prefill(self, rows: list[int], prompts: list[torch.Tensor]) -> torch.Tensor:
         """Prompts[i] behind what sequence rows[i] has cached; their last positions' logits
         [len(rows), V].  One packed pass, or one each for a model class whose masks are
-        built from the positions."""
+        built from the positions or whose rotary tables go by the longest sequence."""
         new = [int(p.numel()) for p in prompts]
         if not new or min(new) < 1:
             raise RuntimeError("a prompt needs at least one token")
         self._check_room(new, rows)
-        if len(rows) > 1 and self._packed_mask is None:
+        keys = {self.lengths[b] + n for b, n in zip(rows, new)}
+        if len(rows) > 1 and (self._packed_mask is None or
+                              (len(keys) > 1 and _rope_by_length(self.model))):
             return torch.cat([self._prefill([b], [p]) for b, p in zip(rows, prompts)])
         lens = [0] * self.B
         for b, n in zip(rows, new):
@@ -556,8 +565,9 @@ class LAPruneLlama:
     def prefill_packed(self, prompts: list[torch.Tensor],
                        rows: list[int] | None = None) -> torch.Tensor:
         """Prefill prompts of different lengths in one pass: prompts[i] (ids [T_i] or
-        [1, T_i]) behind what sequence rows[i] has cached (by default sequence i).
-        Returns each prompt's last-position logits [len(prompts), V]."""
+        [1, T_i]) behind what sequence rows[i] has cached (by default sequence i).  A model
+        whose code could not tell them apart (own masks, rotary tables that go by the longest
+        sequence) takes a pass each.  Returns each prompt's last-position logits [len(prompts), V]."""
         rows = list(range(len(prompts))) if rows is None else [int(b) for b in rows]
         if len(rows) != len(prompts) or len(set(rows)) != len(rows):
             raise RuntimeError("prefill_packed: one sequence of its own per prompt")

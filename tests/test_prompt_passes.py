@@ -80,3 +80,24 @@ def test_a_model_that_makes_its_masks_itself(monkeypatch):
     one = lm.prefill_packed([_ids(30, 3), _ids(20, 4)])
     assert one.shape == (2, VOCAB) and [c[1].lens for c in lm.calls[1:]] == [[30, 0], [0, 20]]
     assert all(_small(c[0]) for c in lm.calls) and lm.lengths == [55, 45]
+
+
+ROPES = [dict(rope_type="dynamic", factor=4.0),
+         dict(rope_type="longrope", factor=4.0, original_max_position_embeddings=64,
+              short_factor=[1.0] * 32, long_factor=[1.0 + i for i in range(32)])]
+
+
+@pytest.mark.parametrize("rope", ROPES, ids=lambda r: r["rope_type"])
+@pytest.mark.parametrize("lens", [(20, 150), (150, 20), (20, 20)])
+def test_rotary_tables_that_go_by_the_length(monkeypatch, rope, lens):
+    """Each prompt is rotated as it would be alone; those of one length still share a pass."""
+    kw = dict(max_position_embeddings=64 if rope["rope_type"] == "dynamic" else 256, rope_scaling=dict(rope))
+    prompts = [_ids(n, n) for n in lens]
+    alone, packed = _lm(monkeypatch, **kw), _lm(monkeypatch, **kw)
+    for b, p in enumerate(prompts):
+        alone.prefill_row(b, p)
+    packed.prefill_packed(prompts)
+    assert len(packed.calls) == (1 if lens[0] == lens[1] else 2)
+    for i in range(2):
+        a, b = (torch.cat([c[2][i] for c in lm.calls], 1) for lm in (alone, packed))
+        assert torch.equal(a, b)
