@@ -505,6 +505,8 @@ class LAPruneLlama:
         """Prompts[i] behind what sequence rows[i] has cached; their last positions' logits
         [len(rows), V].  One packed pass, or one each for a model class whose masks are
         built from the positions or whose rotary tables go by the longest sequence."""
+        if any(p.dim() == 0 or p.numel() != p.shape[-1] for p in prompts):
+            raise RuntimeError("a prompt is one row of ids [T] or [1, T]")
         new = [int(p.numel()) for p in prompts]
         if not new or min(new) < 1:
             raise RuntimeError("a prompt needs at least one token")

@@ -101,3 +101,17 @@ def test_rotary_tables_that_go_by_the_length(monkeypatch, rope, lens):
     for i in range(2):
         a, b = (torch.cat([c[2][i] for c in lm.calls], 1) for lm in (alone, packed))
         assert torch.equal(a, b)
+
+
+def test_a_prompt_is_one_row_of_ids(monkeypatch):
+    """Rows of several are not run together as one prompt."""
+    lm = _lm(monkeypatch)
+    two = _ids(6).view(2, 3)
+    for call in (lambda: lm.prefill_packed([two]), lambda: lm.prefill_row(0, two),
+                 lambda: lm.prefill_shared(two), lambda: lm.prefill_packed([_ids(3), two[None]]),
+                 lambda: lm.prefill_packed([two[0, 0]])):
+        with pytest.raises(RuntimeError, match=r"ids \[T\] or \[1, T\]"):
+            call()
+    assert lm.lengths == [0, 0] and not lm.calls
+    lm.prefill_packed([two[0], two[1:]])
+    assert lm.lengths == [3, 3]
