@@ -39,7 +39,7 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 from ._ops import ops, unwatched
 from .attention import prompt_attention
 from .cache import DecodeKVCache
-from .packed import pack_prompts
+from .packed import MAX_SEQUENCES, pack_prompts
 from .retrieval import DenseDecoder, RetrievalConfig, SparseDecoder, check_step_health
 
 
@@ -498,8 +498,8 @@ class LAPruneLlama:
         return out.logits[:, -1] if isinstance(keep, int) else out.logits[0]
 
     def _packs(self) -> bool:
-        """Whether the packed prompt kernels serve this model."""
-        return self.D in (64, 128, 256) and self.Hq // self.Hkv <= 128
+        """Whether the packed prompt kernels serve this model and batch."""
+        return self.D in (64, 128, 256) and self.Hq // self.Hkv <= 128 and self.B <= MAX_SEQUENCES
 
     def _prefill(self, rows: list[int], prompts: list[torch.Tensor]) -> torch.Tensor:
         """Prompts[i] behind what sequence rows[i] has cached; their last positions' logits
@@ -577,8 +577,8 @@ class LAPruneLlama:
             if not 0 <= b < self.B:
                 raise RuntimeError(f"sequence {b} out of range for batch {self.B}")
         if not self._packs():
-            raise RuntimeError("packed prompts need head dim 64, 128 or 256 and at most 128 query "
-                               "heads per KV head")
+            raise RuntimeError("packed prompts need head dim 64, 128 or 256, at most 128 query heads "
+                               f"per KV head and at most {MAX_SEQUENCES} sequences")
         return self._prefill(rows, prompts)
 
     @torch.no_grad()

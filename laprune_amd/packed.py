@@ -17,6 +17,8 @@ import torch
 from . import _native as N
 from ._ops import ops
 
+MAX_SEQUENCES = 4096  # of one pass (csrc/pack.hip)
+
 
 @functools.lru_cache(1024)
 def prompt_shape(total: int, batch: int, max_keys: int, num_q_heads: int, num_kv_heads: int,

@@ -115,3 +115,18 @@ def test_a_prompt_is_one_row_of_ids(monkeypatch):
     assert lm.lengths == [0, 0] and not lm.calls
     lm.prefill_packed([two[0], two[1:]])
     assert lm.lengths == [3, 3]
+
+
+def test_batches_past_the_packed_tables_run_as_they_came(monkeypatch):
+    """The tables of a pass hold 4096 sequences."""
+    lm = _lm(monkeypatch)
+    assert lm._packs()
+    lm.B = 4096
+    assert lm._packs()
+    lm.B = 4097
+    for st in lm.states:
+        st.cache.lengths = [0] * 4097
+    lm.prefill(_ids(2 * 4097).view(4097, 2))
+    assert len(lm.calls) == 1 and lm.calls[0][1] is None and lm.lengths == [2] * 4097
+    with pytest.raises(RuntimeError, match="4096 sequences"):
+        lm.prefill_packed([_ids(3)])
