@@ -172,7 +172,7 @@ struct TileCopy {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :
                  : "v"(o), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
-                 : "memory");
+                 : "memory", "m0");
   }
 };
 
