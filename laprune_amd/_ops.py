@@ -18,6 +18,7 @@ from pathlib import Path
 
 import torch
 from torch.autograd import forward_ad
+from torch.utils._device import DeviceContext
 
 from . import _native as N
 
@@ -30,14 +31,20 @@ _ops = None
 _compiling, _grad_on = torch.compiler.is_compiling, torch.is_grad_enabled
 _transforms, _modes = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
 _trace = torch._C._get_tracing_state
+_functions, _function_mode = torch._C._len_torch_function_stack, torch._C._get_function_stack_at
+
+
+def _function_modes() -> bool:
+    """Whether a function mode other than a default device looks on."""
+    return any(type(_function_mode(i)) is not DeviceContext for i in range(_functions()))
 
 
 def untraced() -> bool:
     """Whether no compiler, function transform (vmap, jvp), forward-mode level, dispatch
-    mode (fake tensors, op counters) or trace looks at the calling ops, all of which a
-    kernel call would pass by."""
+    mode (fake tensors, op counters), function mode or trace looks at the calling ops, all
+    of which a kernel call would pass by."""
     return not (_compiling() or forward_ad._current_level >= 0 or _transforms() is not None or
-                _modes() or _trace() is not None)
+                _modes() or _trace() is not None or (_functions() and _function_modes()))
 
 
 def unwatched() -> bool:
