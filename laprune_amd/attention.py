@@ -10,7 +10,7 @@ A single query without a mask or down-projections (decode; the reference's
 heads per KV head, K/V rows 16-byte aligned.  Several queries without a mask
 (prefill, with the causal or tail-causal mask of :66-73) run the prompt
 kernel (``lap_prompt_attention``) on rows of the same kind when no gradient is
-needed.  Every other case (an explicit mask, shapes outside the kernels'
+needed and the caller chose no backend (``sdpa_kernel``).  Every other case (an explicit mask, shapes outside the kernels'
 contract) runs ``scaled_dot_product_attention`` exactly as the reference does.
 
 :func:`prompt_attention` is that kernel for packed prompts of different lengths
@@ -69,6 +69,13 @@ def _rows16(t: torch.Tensor) -> bool:
             all(s % 8 == 0 for s in t.stride()[:-1]))
 
 
+def _any_backend() -> bool:
+    """Whether no caller chose among the library's attention kernels (sdpa_kernel(...) or
+    the flags that it sets)."""
+    b = torch.backends.cuda
+    return b.flash_sdp_enabled() and b.mem_efficient_sdp_enabled() and b.math_sdp_enabled()
+
+
 def _prompt_kernel_fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bool:
     """Several queries [B, Hq, Tq, D] at the end of [B, Hkv, Tk, D] keys, for the
     prompt kernel."""
@@ -82,7 +89,7 @@ def _prompt_kernel_fits(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> bo
             k.shape[2] < 1 << 30 and
             # a launch takes less than 2^24 workgroups, each 128 // group tokens of a KV head
             q.shape[0] * k.shape[1] * -(-q.shape[2] // (128 * k.shape[1] // q.shape[1])) < 1 << 24 and
-            max(k.stride(2), v.stride(2)) <= 1 << 24 and untraced() and
+            max(k.stride(2), v.stride(2)) <= 1 << 24 and untraced() and _any_backend() and
             not torch.is_autocast_enabled(q.device.type) and not _needs_grad(q, k, v))
 
 
