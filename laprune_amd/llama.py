@@ -165,10 +165,15 @@ for _f in _DECODE_FORWARDS:
 del _f
 
 
+# Classes whose forward is w * x * rsqrt(mean(x^2) + eps) over the last dimension, by name:
+# a model that has none of one does not load its module.
+_HEAD_NORMS = ("transformers.models.llama.modeling_llama.LlamaRMSNorm",
+               "transformers.models.qwen3.modeling_qwen3.Qwen3RMSNorm")
+
+
 @functools.lru_cache(None)
-def _llama_norm() -> type:
-    from transformers.models.llama.modeling_llama import LlamaRMSNorm
-    return LlamaRMSNorm
+def _head_norm(cls: type) -> bool:
+    return f"{cls.__module__}.{cls.__qualname__}" in _HEAD_NORMS
 
 
 @functools.lru_cache(None)
@@ -384,13 +389,13 @@ class LAPruneLlama:
     def _head_norms(self, attn, q, k, fuse: bool):
         """The layer's norms of q's and k's heads, where it has them: q and k as they are
         and the (weight, eps) of each for the rotation's kernel (``fuse``), or its
-        module's output and None (also for a norm that is not the stock one)."""
+        module's output and None (also for a norm of a class not in _HEAD_NORMS)."""
         out = []
         for mod, x in ((getattr(attn, "q_norm", None), q), (getattr(attn, "k_norm", None), k)):
             w = getattr(mod, "weight", None)
             if mod is None:
                 out.append((x, None))
-            elif (fuse and type(mod) is _llama_norm() and w.numel() == self.D and w.dtype == x.dtype and
+            elif (fuse and _head_norm(type(mod)) and w.numel() == self.D and w.dtype == x.dtype and
                   w.device == x.device and self.D % 16 == 0 and _plain_tensor(w) and _unhooked(mod)):
                 out.append((x, (w, mod.variance_epsilon)))
             else:

@@ -30,3 +30,56 @@ def test_prompts_of_one_and_two_tokens(dev, norms, graph):
         for t in range(2, 5):  # a token that the reference's logits put first, up to their tolerance
             want = _want(ref, out[b, :t])[0].float()
             assert want[out[b, t]] >= want.max() - 2 * TOL * want.abs().max()
+
+
+def _qwen3(dev, D, heads, kv_heads):
+    from transformers import Qwen3Config, Qwen3ForCausalLM
+    torch.manual_seed(2)
+    config = Qwen3Config(vocab_size=1000, hidden_size=512, intermediate_size=1024, num_hidden_layers=3,
+                         num_attention_heads=heads, num_key_value_heads=kv_heads, head_dim=D,
+                         max_position_embeddings=4096, attn_implementation="sdpa")
+    with torch.device(dev):
+        model = Qwen3ForCausalLM(config).to(torch.bfloat16).eval()
+    g = torch.Generator().manual_seed(3)
+    with torch.no_grad():
+        for layer in model.model.layers:
+            for name in ("q_norm", "k_norm"):
+                w = getattr(layer.self_attn, name).weight
+                w.copy_(1 + 0.5 * torch.randn(D, generator=g))
+    return model
+
+
+@pytest.mark.parametrize("D,heads,kv_heads", [(64, 8, 2), (128, 4, 4)])
+def test_a_stock_model_with_head_norms(dev, monkeypatch, D, heads, kv_heads):
+    """Its norms run in the append's launch: packed prompts, eager and captured steps."""
+    import copy
+
+    from test_gpu_packed_llama import _wrap
+
+    from laprune_amd.cache import DecodeKVCache
+    ref = _qwen3(dev, D, heads, kv_heads)
+    lm = _wrap(copy.deepcopy(ref), 2, D=D)
+    fused, plain = [], DecodeKVCache._qk_rope
+
+    def count(self, q, k, v, cos, sin, seq, pos, q_norm, k_norm, q_out):
+        fused.append(q_norm is not None and k_norm is not None)
+        return plain(self, q, k, v, cos, sin, seq, pos, q_norm, k_norm, q_out)
+
+    monkeypatch.setattr(DecodeKVCache, "_qk_rope", count)
+    seqs = [_ids(dev, n, n) for n in (90, 33)]
+    got = lm.prefill_packed([seqs[0][:70], seqs[1]])
+    for g, s in zip(got, (seqs[0][:70], seqs[1])):
+        assert _rel(g, _want(ref, s)[0]) < TOL
+    assert _rel(lm.prefill_row(0, seqs[0][70:]), _want(ref, seqs[0])) < TOL
+    assert fused == [True] * 6
+    more = [_ids(dev, 6, 50 + b) for b in range(2)]
+    for i in range(6):
+        step = (lm.decode if i < 3 else lm.decode_graph)(torch.stack([m[i:i + 1] for m in more]))
+        for b in range(2):
+            assert _rel(step[b:b + 1], _want(ref, torch.cat((seqs[b], more[b][:i + 1])))) < TOL
+    assert len(fused) > 6 and all(fused)
+    # a hook on a norm, or a forward of its own, is not passed by
+    calls = []
+    lm.layers[1].self_attn.q_norm.register_forward_hook(lambda *a: calls.append(1))
+    step = lm.decode(torch.stack([m[:1] for m in more]))
+    assert calls == [1] and fused[-3:] == [True, False, True]
