@@ -222,13 +222,12 @@ def _step_mask(model, batch: int, device):
 def _hands_masks_through(model) -> bool:
     """Whether a 4-D mask reaches the attention layers as it is: the model's code builds
     its masks with transformers' function."""
-    f = inspect.unwrap(type(model.model).forward)
+    f = inspect.unwrap(model.model.forward)
     try:
         from transformers.masking_utils import create_causal_mask
     except ImportError:
         return False
-    return ("forward" not in model.model.__dict__ and
-            getattr(f, "__globals__", {}).get("create_causal_mask") is create_causal_mask)
+    return getattr(f, "__globals__", {}).get("create_causal_mask") is create_causal_mask
 
 
 def _rope_by_length(model) -> bool:

@@ -130,3 +130,18 @@ def test_batches_past_the_packed_tables_run_as_they_came(monkeypatch):
     assert len(lm.calls) == 1 and lm.calls[0][1] is None and lm.lengths == [2] * 4097
     with pytest.raises(RuntimeError, match="4096 sequences"):
         lm.prefill_packed([_ids(3)])
+
+
+@pytest.mark.parametrize("known", [True, False])
+def test_a_wrapped_forward_of_the_model(monkeypatch, known):
+    """One that says what it wraps still hands masks through; any other replacement does not."""
+    import functools
+    from laprune_amd.llama import _hands_masks_through
+    lm = _lm(monkeypatch)
+    inner = lm.model.model.forward
+
+    def outer(*a, **kw):
+        return inner(*a, **kw)
+
+    lm.model.model.forward = functools.update_wrapper(functools.partial(outer), inner) if known else outer
+    assert _hands_masks_through(lm.model) == known
