@@ -589,9 +589,12 @@ int lap_qk_rope_append(const void* q, int64_t q_st, int64_t q_sh,
  * laprune/attention.py:66-73, aq_evaluation.py:279-322): token i of a sequence with
  * `cached` earlier tokens sees keys [0, cached + i],
  *   o[i,h] = sum_t softmax_t(scale * q[i,h].K[b,h/G,t]) V[b,h/G,t]
- * in fp32 but for the weights, which enter the second product in the data type.  A value
- * in a row that a token does not see never reaches it, finite or not; weights that sum
- * to zero give zeros.
+ * in fp32 but for the weights, which enter the second product in the data type: half a
+ * step each (fp16: or 2^-32 of the row's largest, if that is more).  They are relative to a
+ * maximum that may lag behind the row's by up to a factor of 2^8, so the largest is rounded
+ * as well (error of the outputs 1.2 to 1.3 times their own rounding's, 1.15 to 1.2 with exact
+ * maxima).  A value in a row that a token does not see never reaches it, finite or not;
+ * weights that sum to zero give zeros.
  *   tiles non-NULL: q, out [Tq][Hq][D] packed, the tiles of lap_pack_prompts; rows
  *           of no sequence are not written.  tiles NULL: q, out [B][Tq][Hq][D], every
  *           sequence's Tq tokens at the end of Tk keys (Tq <= Tk).
@@ -616,8 +619,8 @@ int lap_prompt_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
  * lap_sparse_attn_decode_ragged read every sequence's own copy).  Keys [0, prefix) are
  * read once, from sequence 0's rows, for all sequences; keys [prefix, len) are each
  * sequence's own.  len = min(plans[b].t_total, T), or T where plans is NULL; a sequence
- * shorter than the prefix sees len keys of it.  Other arguments and the output as
- * lap_dense_attn_decode; q and K/V rows 16-byte aligned, Hq / Hkv up to 128. */
+ * shorter than the prefix sees len keys of it.  Weights are rounded as in
+ * lap_prompt_attention.  Other arguments and the output as lap_dense_attn_decode; q and K/V rows 16-byte aligned, Hq / Hkv up to 128. */
 int lap_shared_attn_decode_workspace_size(int B, int Hq, int Hkv, int D, int T, int prefix,
                                           size_t* bytes);
 int lap_shared_attn_decode(const void* q, int64_t q_sb, int64_t q_sh,

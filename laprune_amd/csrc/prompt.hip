@@ -22,9 +22,9 @@
 //
 // K and V tiles are copied straight into LDS, one tile ahead; 252 registers and 64 KB let
 // two workgroups share a CU, whose products and exponentials overlap.  One prompt of
-// 16384 tokens, 32 query heads on 8, D = 128: 2.07 ms, 1060 TFLOP/s, where a large library
+// 16384 tokens, 32 query heads on 8, D = 128: 2.03 ms, 1085 TFLOP/s, where a large library
 // product reaches 1280 to 1330 on the same card.  The matrix pipe is busy 58 % of the
-// cycles and the card runs at 1.77 GHz under this load: saved cycles come back as a lower
+// cycles and the card runs at 1.79 GHz under this load: saved cycles come back as a lower
 // clock (20 % fewer cycles than an earlier form gave 9 % in time).  LDS reads have no bank
 // conflicts.  Short prompts wait: a tile takes one workgroup 1.2 us, its start, masked
 // tile and end together about 15 us of a 2048-token prompt's 55.
@@ -196,8 +196,12 @@ __device__ __forceinline__ void in_acc(Rows<DT, D>& w) {
 }
 
 // A row's maximum is raised only when a tile exceeds it by more than this, so weights
-// go up to 2^8 before the division by their sum: no rounding differs for it, and the
-// o^T registers are rescaled in few tiles.
+// go up to 2^8 before the division by their sum and the o^T registers are rescaled in
+// few tiles (one prompt of 16384 tokens, 32 heads on 8, D = 128, 2026 us, with exact
+// maxima 2102; 16 heads at D = 256 2423 and 3290).  The price: with an exact maximum the
+// largest weight is 1 and not rounded, so the outputs' error against 64 bits (256 to 8192
+// tokens, scores of deviation 1.5) is 1.15 to 1.19 times that of their own rounding, and
+// 1.19 to 1.32 so.
 constexpr float kSlack = 8.f;
 // The exponent m that a row's weights are relative to lies this far below its maximum.  fp16
 // has no relative steps below 2^-14 and nothing below 2^-25: with weights of up to 2^15 (and the
@@ -236,7 +240,7 @@ __device__ __forceinline__ uint32_t pinned(uint32_t at) {
 // The three parts of a tile's work.  Buffers are named by their byte offset from the
 // first one.
 
-// Scores of the 64 keys of the K buffer at kb: their operands, and the products.
+// Scores of the keys of the K buffer at kb: their operands, and the products.
 template <int D>
 using KeyOps = i16x8[bn<D>() / 32][D / 16];
 template <int D>
@@ -317,7 +321,7 @@ __device__ __forceinline__ void weights(Rows<DT, D>& w, Scores<D>& s, Weights<D>
   w.l += sum[0] + sum[1];
 }
 
-// o^T += V^T P^T of the 64 rows of the V buffer at vb.
+// o^T += V^T P^T of the rows of the V buffer at vb.
 template <int DT, int D>
 __device__ __forceinline__ void values(Rows<DT, D>& w, const LaneAddr<D>& la, uint32_t vb,
                                        const Weights<D>& pk) {
@@ -814,7 +818,10 @@ int check_heads(const char* fn, int Hq, int Hkv, int D) {
 // one round of workgroups with parts of at least 512 keys was 10 % (16384 tokens of 2 heads
 // on 2, 3 parts 172 us, 1 301, 4 202; 1200 tokens behind 64336, 32 heads on 8, 6 parts 1278,
 // 1 1651; 2048 tokens of 8 heads on 4, D = 256, 3 parts 48, 4 66, 1 80; 2048 tokens of 32
-// heads on 8, 1 part 52, 2 66).
+// heads on 8, 1 part 52, 2 66).  In all of them a batch's sequences had one cached length:
+// every tile counts with max_keys, so one long cache among short ones gets too few parts
+// (64 turns of 32 tokens, 32 heads on 8, one behind 131040 and 63 behind 200: 1 part, 2382
+// us, where they take 142 and 21 in passes of their own).
 int prompt_splits(int64_t items, double fresh, int max_keys, int D) {
   if (items == 0 || max_keys == 0) return 1;
   const int64_t slots = D == 256 ? 256 : 512;  // workgroups that run at a time
@@ -946,6 +953,9 @@ namespace {
 // workgroups run at a time; a workgroup's start, its first copies and its part of the
 // merge cost about as much as six tiles of 64 keys (64 sequences
 // behind 2000 tokens with up to 2000 of their own: 54.1 us, 70.6 if counted as three).
+// Every sequence counts as T keys long; where its length is on the device T is the caches'
+// capacity, and room in them costs parts (16 sequences behind 16384 tokens with up to 883 of
+// their own: 24.9 us at T = 17267, 40.8, 49.9 and 89.5 at two, four and eight times as many).
 struct SharedShape {
   int bt, pblocks, per, psplit, nsplit;
 };

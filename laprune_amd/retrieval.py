@@ -425,7 +425,8 @@ class DenseDecoder:
 
         shared_prefix: the first so many tokens are the same in every sequence;
         their rows of sequence 0 are read once for the whole batch, and the other
-        sequences' copies not at all."""
+        sequences' copies not at all.  Roundings as in
+        :func:`laprune_amd.attention.prompt_attention`."""
         B, Hkv, D = self.B, self.Hkv, self.D
         T = keys.shape[2]
         rows = _per_row(lengths, B, "lengths")
